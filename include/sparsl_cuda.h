@@ -413,6 +413,148 @@ int sparsl_dev_scan_stats(sparsl_dev *dev, uint64_t *repaired, uint64_t *segment
 int sparsl_dev_assoc_scan_noalloc(int ordinal, const float *d_in, uint64_t n, float *d_out,
                                   void *stream, uint64_t timeout_ms);
 
+/* ---- sequence operators over device arrays (extension) -------------------- */
+/* The recurrences of sequence models beside assoc_scan: the short causal
+ * convolution, the selective state space scan (one affine map per channel,
+ * state and token, chosen by the input) and layer norm; each for prompts and
+ * training with its gradients, the first two also for one token of each
+ * running sequence.
+ *
+ * Conventions
+ *  - Token arrays are rows of `channels` values (f32, binary16 or bfloat16:
+ *    dtype 0, 1, 2), the channels next to each other; a row's stride is in
+ *    elements, so a column range of a wider array is a token array.
+ *  - The sequences' tokens follow one another.  seq_ptr (device, n_seq + 1,
+ *    ascending, at most `tokens`) says where each begins; NULL stands for
+ *    n_seq sequences of tokens / n_seq tokens each.  Empty sequences are
+ *    allowed.  Rows in front of the first sequence and behind the last are
+ *    neither read nor written.
+ *  - slots (device, n_seq): the row of the state arrays that sequence i uses;
+ *    NULL: row i.  A slot outside [0, n_slots) is none: the sequence starts
+ *    from zero and leaves no state (in a step, its row is skipped).  Two
+ *    sequences of a call must not name the same slot: which of them it then
+ *    holds is not specified.
+ *  - state: what each sequence starts from; NULL: zeros.  resume (device,
+ *    n_seq bytes): a 0 starts that sequence from zero instead; NULL: all
+ *    resume.  final_state: where its state behind the last token goes, also
+ *    for an empty sequence; it may be `state` itself (a pool updated in
+ *    place) or another array, not a part of it.
+ *  - Sums, states and gradients of parameters are f32; token outputs are
+ *    rounded once.  Results do not change from run to run.
+ *  - Work is only enqueued on `stream` (cudaStream_t, NULL = the device's
+ *    own); nothing is allocated and nothing waits, so calls can be captured
+ *    into a CUDA graph.  Workspaces are the caller's (16-byte aligned, of the
+ *    size that the _workspace function gives for the same sizes) and must not
+ *    be shared by calls that may run at the same time.
+ *  - Every array must be device memory of this GPU inside one allocation
+ *    (else SPARSL_ERR_INVALID).  An output that overlaps an input or another
+ *    output is refused (SPARSL_ERR_INVALID), except a state updated in place;
+ *    sizes that do not fit one another give SPARSL_ERR_LENGTH. */
+typedef struct {
+  uint64_t tokens, n_seq;
+  const int32_t *seq_ptr;
+  const int32_t *slots;
+  const uint8_t *resume;
+  uint64_t n_slots;
+} sparsl_seqs;
+/* Rows of a token array: the first value and the elements from row to row. */
+typedef struct {
+  void *p;
+  uint64_t stride;
+} sparsl_rows;
+/* u[t, c] = bias[c] + sum_k weight[c, k] x[t - (width - 1) + k, c];
+ * y = u, or u sigmoid(u) with silu.  weight [channels, width], bias [channels]
+ * or NULL: f32 (params_f32) or of dtype.  width 2..4.  state, final_state and
+ * their gradients: [n_slots, width - 1, channels] of dtype, the inputs before
+ * the next token, oldest first. */
+typedef struct {
+  sparsl_seqs seqs;
+  int32_t dtype, params_f32, silu;
+  uint32_t channels, width;
+  sparsl_rows x, y;
+  const void *weight, *bias, *state;
+  void *final_state;
+  /* backward: dx, dweight [channels, width], dbias [channels] or NULL (f32);
+   * dstate (NULL: not wanted) is the gradient of `state`, dfinal_state (NULL:
+   * zero) that of the final state. */
+  sparsl_rows dy, dx;
+  float *dweight, *dbias;
+  void *dstate;
+  const void *dfinal_state;
+  void *workspace;
+  uint64_t workspace_bytes;
+} sparsl_conv_args;
+int sparsl_dev_causal_conv_device(sparsl_dev *dev, const sparsl_conv_args *args, void *stream);
+/* slots and resume must be NULL here: row i of the state arrays is sequence i's. */
+int sparsl_dev_causal_conv_backward_device(sparsl_dev *dev, const sparsl_conv_args *args, void *stream);
+uint64_t sparsl_causal_conv_backward_workspace(uint64_t tokens, uint64_t channels, uint32_t width);
+/* One token of each of n_seq sequences: x and y have n_seq rows; final_state
+ * holds the states, updated in place. */
+int sparsl_dev_causal_conv_step_device(sparsl_dev *dev, const sparsl_conv_args *args, void *stream);
+
+/* s = dt + dt_bias, through log(1 + e^v) with softplus;
+ * h[c, n] <- exp(s a[c, n]) h[c, n] + s b[n] x;
+ * y = sum_n c[n] h[c, n] + d[c] x, times z sigmoid(z) with z.
+ * a [channels, states], d, dt_bias [channels] or NULL: f32.  b, c: per token
+ * `groups` runs of `states` values (a run every b_group / c_group elements);
+ * channels / groups neighbouring channels share a run.  states 1..64.
+ * state, final_state and their gradients: f32 [n_slots, channels, states]. */
+typedef struct {
+  sparsl_seqs seqs;
+  int32_t dtype, softplus;
+  uint32_t channels, states, groups, reserved;
+  sparsl_rows x, dt, z, b, c, y;
+  uint64_t b_group, c_group;
+  const float *a, *d, *dt_bias, *state;
+  float *final_state;
+  /* States kept for the backward pass (sparsl_selective_scan_checkpoints
+   * bytes), written by the forward call and read by the backward call on the
+   * same inputs; NULL in a forward call that no backward call follows. */
+  void *checkpoints;
+  uint64_t checkpoint_bytes;
+  /* backward: dd and ddt_bias may be NULL, dz goes with z; da [channels,
+   * states], dd, ddt_bias [channels] in f32; db, dc laid out as b and c. */
+  sparsl_rows dy, dx, ddt, dz, db, dc;
+  uint64_t db_group, dc_group;
+  float *da, *dd, *ddt_bias, *dstate;
+  const float *dfinal_state;
+  void *workspace;
+  uint64_t workspace_bytes;
+} sparsl_scan_args;
+int sparsl_dev_selective_scan_device(sparsl_dev *dev, const sparsl_scan_args *args, void *stream);
+uint64_t sparsl_selective_scan_workspace(uint64_t tokens, uint64_t channels, uint32_t states,
+                                         uint64_t n_seq, uint32_t groups);
+uint64_t sparsl_selective_scan_checkpoints(uint64_t tokens, uint64_t channels, uint32_t states);
+/* slots and resume must be NULL here: row i of the state arrays is sequence i's. */
+int sparsl_dev_selective_scan_backward_device(sparsl_dev *dev, const sparsl_scan_args *args, void *stream);
+uint64_t sparsl_selective_scan_backward_workspace(uint64_t tokens, uint64_t channels, uint32_t states,
+                                                  uint64_t n_seq, uint32_t groups);
+/* One token of each of n_seq sequences: the token arrays have n_seq rows;
+ * final_state holds the states, updated in place. */
+int sparsl_dev_selective_scan_step_device(sparsl_dev *dev, const sparsl_scan_args *args, void *stream);
+
+/* y = (x - mean) rstd weight + bias over each row's channels, rstd =
+ * 1 / sqrt(variance + eps).  weight, bias [channels] or NULL (1 and 0), f32
+ * (params_f32) or of dtype; mean, rstd [rows] f32 or NULL in the forward call.
+ * backward: mean and rstd as the forward call wrote them; dweight, dbias
+ * [channels] f32 or NULL. */
+typedef struct {
+  uint64_t rows, channels;
+  int32_t dtype, params_f32;
+  sparsl_rows x, y;
+  const void *weight, *bias;
+  float *mean, *rstd;
+  float eps;
+  uint32_t reserved;
+  sparsl_rows dy, dx;
+  float *dweight, *dbias;
+  void *workspace;
+  uint64_t workspace_bytes;
+} sparsl_norm_args;
+int sparsl_dev_layer_norm_device(sparsl_dev *dev, const sparsl_norm_args *args, void *stream);
+int sparsl_dev_layer_norm_backward_device(sparsl_dev *dev, const sparsl_norm_args *args, void *stream);
+uint64_t sparsl_layer_norm_backward_workspace(uint64_t rows, uint64_t channels);
+
 /* ---- pinned host memory (for end-to-end copies at DMA speed) ------------- */
 void *sparsl_host_alloc(uint64_t bytes);
 void sparsl_host_free(void *p);

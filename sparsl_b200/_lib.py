@@ -37,6 +37,51 @@ class Shape(ctypes.Structure):
                 ("nnz", u64), ("max_row_nnz", u64)]
 
 
+u32 = ctypes.c_uint32
+i32t = ctypes.c_int32
+
+
+class Seqs(ctypes.Structure):
+    """``sparsl_seqs``."""
+
+    _fields_ = [("tokens", u64), ("n_seq", u64), ("seq_ptr", vp), ("slots", vp), ("resume", vp), ("n_slots", u64)]
+
+
+class Rows(ctypes.Structure):
+    """``sparsl_rows``."""
+
+    _fields_ = [("p", vp), ("stride", u64)]
+
+
+class ConvArgs(ctypes.Structure):
+    """``sparsl_conv_args``."""
+
+    _fields_ = [("seqs", Seqs), ("dtype", i32t), ("params_f32", i32t), ("silu", i32t), ("channels", u32), ("width", u32),
+                ("x", Rows), ("y", Rows), ("weight", vp), ("bias", vp), ("state", vp), ("final_state", vp), ("dy", Rows),
+                ("dx", Rows), ("dweight", vp), ("dbias", vp), ("dstate", vp), ("dfinal_state", vp), ("workspace", vp),
+                ("workspace_bytes", u64)]
+
+
+class ScanArgs(ctypes.Structure):
+    """``sparsl_scan_args``."""
+
+    _fields_ = [("seqs", Seqs), ("dtype", i32t), ("softplus", i32t), ("channels", u32), ("states", u32), ("groups", u32),
+                ("reserved", u32), ("x", Rows), ("dt", Rows), ("z", Rows), ("b", Rows), ("c", Rows), ("y", Rows),
+                ("b_group", u64), ("c_group", u64), ("a", vp), ("d", vp), ("dt_bias", vp), ("state", vp),
+                ("final_state", vp), ("checkpoints", vp), ("checkpoint_bytes", u64), ("dy", Rows), ("dx", Rows),
+                ("ddt", Rows), ("dz", Rows), ("db", Rows), ("dc", Rows), ("db_group", u64), ("dc_group", u64), ("da", vp),
+                ("dd", vp), ("ddt_bias", vp), ("dstate", vp), ("dfinal_state", vp), ("workspace", vp),
+                ("workspace_bytes", u64)]
+
+
+class NormArgs(ctypes.Structure):
+    """``sparsl_norm_args``."""
+
+    _fields_ = [("rows", u64), ("channels", u64), ("dtype", i32t), ("params_f32", i32t), ("x", Rows), ("y", Rows),
+                ("weight", vp), ("bias", vp), ("mean", vp), ("rstd", vp), ("eps", f32), ("reserved", u32), ("dy", Rows),
+                ("dx", Rows), ("dweight", vp), ("dbias", vp), ("workspace", vp), ("workspace_bytes", u64)]
+
+
 # name -> (restype, argtypes); every symbol include/*.h declares.
 SIGNATURES = {
     "sparsl_last_error": (ctypes.c_char_p, []),
@@ -122,6 +167,19 @@ SIGNATURES = {
     "sparsl_dev_wait": (i32, [vp]),
     "sparsl_dev_scan_stats": (i32, [vp, ctypes.POINTER(u64), ctypes.POINTER(u64)]),
     "sparsl_dev_assoc_scan_noalloc": (i32, [i32, vp, u64, vp, vp, u64]),
+    "sparsl_dev_causal_conv_device": (i32, [vp, vp, vp]),
+    "sparsl_dev_causal_conv_backward_device": (i32, [vp, vp, vp]),
+    "sparsl_causal_conv_backward_workspace": (u64, [u64, u64, u32]),
+    "sparsl_dev_causal_conv_step_device": (i32, [vp, vp, vp]),
+    "sparsl_dev_selective_scan_device": (i32, [vp, vp, vp]),
+    "sparsl_selective_scan_workspace": (u64, [u64, u64, u32, u64, u32]),
+    "sparsl_selective_scan_checkpoints": (u64, [u64, u64, u32]),
+    "sparsl_dev_selective_scan_backward_device": (i32, [vp, vp, vp]),
+    "sparsl_selective_scan_backward_workspace": (u64, [u64, u64, u32, u64, u32]),
+    "sparsl_dev_selective_scan_step_device": (i32, [vp, vp, vp]),
+    "sparsl_dev_layer_norm_device": (i32, [vp, vp, vp]),
+    "sparsl_dev_layer_norm_backward_device": (i32, [vp, vp, vp]),
+    "sparsl_layer_norm_backward_workspace": (u64, [u64, u64]),
     "sparsl_host_alloc": (vp, [u64]),
     "sparsl_host_free": (None, [vp]),
     "sparsl_device_alloc": (vp, [vp, u64]),

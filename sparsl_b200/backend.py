@@ -23,6 +23,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import Shape
+from .sequence import SequenceOps
 
 # --------------------------------------------------------------------------
 # Backend identity and availability (mod.rs:60-202)
@@ -365,7 +366,7 @@ def spikes_to_f32(words, n: int) -> np.ndarray:
 # --------------------------------------------------------------------------
 
 
-class Device:
+class Device(SequenceOps):
     """A handle to a CUDA device that was available when it was opened."""
 
     def __init__(self, backend: Backend, handle, ordinal: int):

@@ -1051,6 +1051,7 @@ int check_device_array(const void* p, uint64_t bytes, int ordinal, const char* w
   return check_device_span(p, bytes, ordinal, what);
 }
 std::string describe_device_error(uint32_t bits) { return describe_dev_err(bits); }
+int device_ordinal(const sparsl_dev* d) { return d->ordinal; }
 }  // namespace sparsl
 
 extern "C" {

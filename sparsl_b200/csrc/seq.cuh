@@ -1,0 +1,214 @@
+// Sequence operators: the short causal convolution, the selective state space
+// scan and layer norm over token arrays [tokens, channels].
+//
+// Tokens of all sequences lie one after another; sequence i holds the tokens
+// [seq_ptr[i], seq_ptr[i + 1]), or n_seq equal runs without seq_ptr.  Every
+// kernel clamps what it reads from seq_ptr to [0, tokens] and treats a slot
+// outside [0, n_slots) as none, so no content of those device arrays leads an
+// access out of the buffers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace sparsl {
+
+struct SeqView {
+  uint64_t tokens;
+  uint64_t n_seq;
+  uint64_t run;            // tokens of each sequence when seq_ptr is null
+  const int32_t* seq_ptr;  // n_seq + 1, or null
+  const int32_t* slots;    // n_seq, or null: sequence i keeps its state in row i
+  const uint8_t* resume;   // n_seq, or null: all continue from their state
+  uint64_t n_slots;
+
+  __device__ __forceinline__ int64_t begin(int64_t i) const {
+    if (!seq_ptr) return i * (int64_t)run;
+    const int64_t v = __ldg(seq_ptr + i);
+    return v < 0 ? 0 : (v > (int64_t)tokens ? (int64_t)tokens : v);
+  }
+  // The last sequence that begins at or before token t (-1: none).
+  __device__ __forceinline__ int64_t of(int64_t t) const {
+    if (!seq_ptr) {
+      const int64_t i = run ? t / (int64_t)run : (int64_t)n_seq;
+      return i < (int64_t)n_seq ? i : (int64_t)n_seq;
+    }
+    int64_t lo = 0, hi = (int64_t)n_seq + 1;  // the first entry above t lies in [lo, hi]
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (begin(mid) <= t) lo = mid + 1; else hi = mid;
+    }
+    return lo - 1;
+  }
+  // The first sequence that begins at or behind token t (n_seq: none).
+  __device__ __forceinline__ int64_t first_from(int64_t t) const {
+    if (!seq_ptr) {
+      if (!run) return t > 0 ? (int64_t)n_seq : 0;
+      const int64_t i = (t + (int64_t)run - 1) / (int64_t)run;
+      return i < (int64_t)n_seq ? i : (int64_t)n_seq;
+    }
+    int64_t lo = 0, hi = (int64_t)n_seq;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (begin(mid) < t) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+  }
+  // The state row of sequence i, or -1.
+  __device__ __forceinline__ int64_t slot(int64_t i) const {
+    const int64_t s = slots ? (int64_t)__ldg(slots + i) : i;
+    return s >= 0 && s < (int64_t)n_slots ? s : -1;
+  }
+  __device__ __forceinline__ bool resumes(int64_t i) const { return !resume || __ldg(resume + i) != 0; }
+};
+
+enum SeqType : int { SEQ_F32 = 0, SEQ_F16 = 1, SEQ_BF16 = 2 };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// A parameter (weight, bias) is f32 or has the tokens' type.
+template <class T>
+__device__ __forceinline__ float load_param(const void* p, bool f32, uint64_t i) {
+  return f32 ? __ldg(reinterpret_cast<const float*>(p) + i) : to_f32(reinterpret_cast<const T*>(p)[i]);
+}
+
+// V values of type T as one access where V * sizeof(T) is 4, 8 or 16 bytes.
+template <class T, int V>
+struct alignas(sizeof(T) * V) Pack {
+  T v[V];
+};
+template <class T, int V>
+__device__ __forceinline__ void load_pack(const T* p, float (&out)[V]) {
+  const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = to_f32(k.v[i]);
+}
+template <class T, int V>
+__device__ __forceinline__ void store_pack(T* p, const float (&in)[V]) {
+  Pack<T, V> k;
+#pragma unroll
+  for (int i = 0; i < V; ++i) k.v[i] = from_f32<T>(in[i]);
+  *reinterpret_cast<Pack<T, V>*>(p) = k;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^v and 1/v by the special function unit (relative error below 2^-22 and
+// 2^-23): the sums they enter are rounded at 2^-24 a step, and the outputs
+// they reach at most at that of f32.
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float sigmoid(float v) { return rcp(1.0f + ex2(-kLog2e * v)); }
+
+// Column sums of part[rows, cols]: columns below `split` into out, the rest into more (may be null).
+cudaError_t launch_reduce_rows(const float* part, uint64_t rows, uint64_t cols, uint64_t split, float* out, float* more,
+                               cudaStream_t s);
+
+// ---- the short causal convolution (conv.cu) ----
+struct ConvArgs {
+  SeqView seq;
+  int type;
+  uint32_t channels, width;
+  bool silu, params_f32;
+  const void* x;
+  uint64_t x_stride;
+  const void* w;     // [channels, width]
+  const void* bias;  // [channels] or null
+  void* y;
+  uint64_t y_stride;
+  const void* state;  // [n_slots, width - 1, channels] or null
+  void* final_state;
+  // backward
+  const void* dy;
+  uint64_t dy_stride;
+  void* dx;
+  uint64_t dx_stride;
+  float* dw;
+  float* dbias;
+  void* dstate;
+  const void* dfinal;
+  float* part;
+};
+size_t conv_backward_bytes(uint64_t tokens, uint64_t channels, uint32_t width);
+cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s);
+cudaError_t launch_conv_backward(const ConvArgs& a, cudaStream_t s);
+cudaError_t launch_conv_step(const ConvArgs& a, cudaStream_t s);
+
+// ---- the selective scan (sscan.cu) ----
+struct SscanArgs {
+  SeqView seq;
+  int type;
+  uint32_t channels, states, groups;
+  bool softplus;
+  const void *x, *dt, *z, *b, *c;
+  uint64_t x_stride, dt_stride, z_stride, b_stride, c_stride, b_group, c_group;
+  const float *a, *d, *dt_bias;
+  void* y;
+  uint64_t y_stride;
+  const float* state;  // [n_slots, channels, states] or null
+  float* final_state;
+  float* marks;  // states before every kMarkEvery-th token, or null
+  void* work;
+  // backward
+  const void* dy;
+  uint64_t dy_stride;
+  void *dx, *ddt, *dz, *db, *dc;
+  uint64_t dx_stride, ddt_stride, dz_stride, db_stride, dc_stride, db_group, dc_group;
+  float *da, *dd, *ddt_bias;
+  float* dstate;
+  const float* dfinal;
+};
+constexpr uint32_t kMaxStates = 64;
+size_t sscan_bytes(uint64_t tokens, uint64_t channels, uint32_t states, uint64_t n_seq, uint32_t groups);
+size_t sscan_backward_bytes(uint64_t tokens, uint64_t channels, uint32_t states, uint64_t n_seq, uint32_t groups);
+size_t sscan_mark_bytes(uint64_t tokens, uint64_t channels, uint32_t states);
+cudaError_t launch_sscan(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_backward(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_step(const SscanArgs& a, cudaStream_t s);
+
+// ---- layer norm (norm.cu) ----
+struct NormArgs {
+  int type;
+  bool params_f32;
+  uint64_t rows, channels;
+  const void* x;
+  uint64_t x_stride;
+  const void *w, *bias;
+  float eps;
+  void* y;
+  uint64_t y_stride;
+  float *mean, *rstd;
+  const void* dy;
+  uint64_t dy_stride;
+  void* dx;
+  uint64_t dx_stride;
+  float *dw, *dbias;
+  float* part;
+};
+size_t norm_backward_bytes(uint64_t rows, uint64_t channels);
+cudaError_t launch_norm(const NormArgs& a, cudaStream_t s);
+cudaError_t launch_norm_backward(const NormArgs& a, cudaStream_t s);
+
+}  // namespace sparsl
