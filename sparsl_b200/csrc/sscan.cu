@@ -17,51 +17,131 @@
 namespace sparsl {
 namespace {
 
-constexpr int kAhead = 8;  // tokens loaded at a time
+constexpr int kAhead = 8;  // tokens in a batch: the next batch's rows are loaded while one is computed
 
-template <class T>
-struct Raw3 {
-  T x[kAhead], dt[kAhead], z[kAhead];
+// One token of NS states, two at a time: h <- e h + (s x) B.
+template <int NS, bool FULL>
+__device__ __forceinline__ void advance(float s, float sx, const float* b, const f32x2 (&a2)[NS / 2], uint32_t n0, uint32_t N,
+                                        f32x2 (&h)[NS / 2]) {
+  const f32x2 ss = pair(s, s), xx = pair(sx, sx);
+#pragma unroll
+  for (int j = 0; j < NS / 2; j += 2) {
+    const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(b + 2 * j);
+    f32x2 add0 = mul2(xx, bb.x), add1 = mul2(xx, bb.y);
+    if (!FULL) {  // an infinite x must not reach a state that does not exist
+      float lo, hi;
+      unpair(add0, lo, hi);
+      add0 = pair(n0 + 2 * j < N ? lo : 0.f, n0 + 2 * j + 1 < N ? hi : 0.f);
+      unpair(add1, lo, hi);
+      add1 = pair(n0 + 2 * j + 2 < N ? lo : 0.f, n0 + 2 * j + 3 < N ? hi : 0.f);
+    }
+    h[j] = fma2(ex2_2(mul2(ss, a2[j])), h[j], add0);
+    h[j + 1] = fma2(ex2_2(mul2(ss, a2[j + 1])), h[j + 1], add1);
+  }
+}
+
+template <int NS, bool FULL>
+__device__ __forceinline__ void load_pairs(const float* p, uint32_t n0, uint32_t N, f32x2 (&h)[NS / 2], float scale = 1.f) {
+  float v[NS];
+  load_states<NS, FULL>(p, n0, N, v);
+#pragma unroll
+  for (int j = 0; j < NS / 2; ++j) h[j] = pair(v[2 * j] * scale, v[2 * j + 1] * scale);
+}
+template <int NS, bool FULL>
+__device__ __forceinline__ void store_pairs(float* p, uint32_t n0, uint32_t N, const f32x2 (&h)[NS / 2]) {
+  float v[NS];
+#pragma unroll
+  for (int j = 0; j < NS / 2; ++j) unpair(h[j], v[2 * j], v[2 * j + 1]);
+  store_states<NS, FULL>(p, n0, N, v);
+}
+template <int M>
+__device__ __forceinline__ void zero_pairs(f32x2 (&h)[M]) {
+#pragma unroll
+  for (int j = 0; j < M; ++j) h[j] = 0ull;
+}
+
+// The rows of B, and behind each those of C (R = 2), of a tile's tokens: every
+// thread fetches some values of the next tile while one is computed, and puts
+// them, as f32, into the other of two buffers.
+template <class T, int NP, int R>
+struct StageBC {
+  static constexpr int kEach = (kScanTile * R * NP + kScanThreads - 1) / kScanThreads;
+  T v[kEach];
+  uint32_t got;
+  __device__ __forceinline__ void fetch(const SscanArgs& a, uint32_t group, int64_t tb, uint32_t live) {
+    got = 0;
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      const uint32_t i = q * kScanThreads + threadIdx.x, n = i % NP, which = i / NP % R, k = i / (NP * R);
+      if (k < (uint32_t)kScanTile && (live >> k & 1) && n < a.states) {
+        const T* p = reinterpret_cast<const T*>(which ? a.c : a.b);
+        v[q] = p[(uint64_t)(tb + k) * (which ? a.c_stride : a.b_stride) + (uint64_t)group * (which ? a.c_group : a.b_group) + n];
+        got |= 1u << q;
+      }
+    }
+  }
+  __device__ __forceinline__ void put(float* sh) const {
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      const uint32_t i = q * kScanThreads + threadIdx.x;
+      if (i < kScanTile * R * NP) sh[i] = got >> q & 1 ? to_f32(v[q]) : 0.f;
+    }
+  }
 };
 
-// B and (BOTH) C of the tokens of a tile from tb on that `live` names, as f32
-// in shared memory; what does not exist is 0.
-template <class T, int NP, bool BOTH>
-__device__ __forceinline__ void stage_bc(const SscanArgs& a, uint32_t group, int64_t tb, uint32_t live,
-                                         float (*sh)[2][NP]) {
-  constexpr int kRows = BOTH ? 2 : 1;
-  for (int i = threadIdx.x; i < kScanTile * kRows * NP; i += kScanThreads) {
-    const uint32_t n = i % NP, which = i / NP % kRows, k = i / (NP * kRows);
-    const int64_t t = tb + k;
-    float v = 0.f;
-    if ((live >> k & 1) && n < a.states) {
-      const T* p = reinterpret_cast<const T*>(which ? a.c : a.b);
-      v = to_f32(p[(uint64_t)t * (which ? a.c_stride : a.b_stride) + (uint64_t)group * (which ? a.c_group : a.b_group) + n]);
+// Rows of a batch, one token in LP of them per lane: the lanes that share a
+// channel divide a token's own work (step, gate, output) among them.
+template <class T, int LP>
+struct Batch {
+  static constexpr int kOwn = kAhead / LP;
+  T x[kOwn], dt[kOwn], z[kOwn];
+  template <bool GATE>
+  __device__ __forceinline__ void load(const T* px, const T* pdt, const T* pz, const SscanArgs& a) {
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      x[j] = *px;
+      dt[j] = *pdt;
+      px += LP * a.x_stride;
+      pdt += LP * a.dt_stride;
+      if (GATE) {
+        z[j] = *pz;
+        pz += LP * a.z_stride;
+      }
     }
-    sh[k][which][n] = v;
   }
+};
+
+template <int LP>
+__device__ __forceinline__ float from_lane(float v, int q) {
+  if constexpr (LP == 1) return v;
+  else return __shfl_sync(0xffffffffu, v, q, LP);
+}
+// o[q] of LP lanes: lane q gets the sum of their o[q].
+template <int LP>
+__device__ __forceinline__ float scatter_sum(float (&o)[LP], uint32_t part) {
+#pragma unroll
+  for (int w = LP / 2; w >= 1; w /= 2) {
+    const bool up = part & w;
+#pragma unroll
+    for (int j = 0; j < w; ++j) {
+      const float send = up ? o[j] : o[j + w], keep = up ? o[j + w] : o[j];
+      o[j] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+    }
+  }
+  return o[0];
 }
 
-// One token of NS states: h <- a h + (s x) B.
-template <int NS, bool FULL>
-__device__ __forceinline__ void advance(float s, float sx, const float* b, const float (&a2)[NS], uint32_t n0, uint32_t N,
-                                        float (&h)[NS]) {
-#pragma unroll
-  for (int j = 0; j < NS; ++j) {
-    float add = sx * b[j];
-    if (!FULL && n0 + j >= N) add = 0.f;  // an infinite x must not reach a state that does not exist
-    h[j] = __fmaf_rn(ex2(s * a2[j]), h[j], add);
-  }
-}
+__device__ __forceinline__ uint32_t first_bits(int64_t n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
 
 // The state that a chunk hands to the next one: its last sequence's, from that
 // sequence's start in it or from zero.
 template <class T, int NS, int LP, bool FULL>
-__global__ void __launch_bounds__(kScanThreads) sscan_chunk_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
+__global__ void __launch_bounds__(kScanThreads, 4) sscan_chunk_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
   constexpr int NP = NS * LP;
-  __shared__ __align__(16) float bc[kScanTile][2][NP];
+  __shared__ __align__(16) float bc[2][kScanTile][NP];
   const uint32_t N = a.states;
   const ScanLane<NS, LP> me(a.channels, a.groups, p.per_group, blockIdx.x % p.ctiles);
+  const uint32_t part = threadIdx.x % LP;
   const int64_t chunk = blockIdx.x / p.ctiles;
   const int64_t t0 = chunk * (int64_t)p.len, t1 = min(t0 + (int64_t)p.len, (int64_t)a.seq.tokens);
   const int64_t seq = a.seq.of(t1 - 1);
@@ -70,45 +150,67 @@ __global__ void __launch_bounds__(kScanThreads) sscan_chunk_kernel(SscanArgs a, 
   const bool spans = any && end > t1 && begin < t1;
   if (threadIdx.x == 0 && blockIdx.x % p.ctiles == 0) w.cut[chunk] = !spans ? 2 : begin >= t0 ? 1 : 0;
   if (!spans) return;
-  float h[NS], a2[NS];
-  load_states<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2);
-#pragma unroll
-  for (int j = 0; j < NS; ++j) a2[j] *= kLog2e;
-  zero_states(h);
+  f32x2 h[NS / 2], a2[NS / 2];
+  load_pairs<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2, kLog2e);
+  zero_pairs(h);
   const uint64_t row = ((uint64_t)chunk * a.channels + me.c) * N;
   if (begin >= t0 && a.state) {
     const int64_t slot = a.seq.resumes(seq) ? a.seq.slot(seq) : -1;
-    if (slot >= 0) load_states<NS, FULL>(a.state + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, h);
-    if (w.start && me.valid) store_states<NS, FULL>(w.start + row, me.n0, N, h);
+    if (slot >= 0) load_pairs<NS, FULL>(a.state + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, h);
+    if (w.start && me.valid) store_pairs<NS, FULL>(w.start + row, me.n0, N, h);
   }
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
   const T* x = reinterpret_cast<const T*>(a.x) + me.c;
   const T* dt = reinterpret_cast<const T*>(a.dt) + me.c;
   float sum = 0.f;
-  for (int64_t tb = max(begin, t0); tb < t1; tb += kScanTile) {
-    __syncthreads();
-    stage_bc<T, NP, false>(a, me.group, tb, t1 - tb >= 32 ? ~0u : (1u << (t1 - tb)) - 1, bc);
-    __syncthreads();
-    for (int k = 0; k < kScanTile; k += kAhead) {
-      T xr[kAhead], dr[kAhead];
+  StageBC<T, NP, 1> stage;
+  Batch<T, LP> now, next;
+  const int64_t from = max(begin, t0);
+  stage.fetch(a, me.group, from, first_bits(t1 - from));
+  stage.put(&bc[0][0][0]);
+  const T* px = x + (uint64_t)(from + part) * a.x_stride;
+  const T* pdt = dt + (uint64_t)(from + part) * a.dt_stride;
+  if (t1 - from >= kAhead) next.template load<false>(px, pdt, nullptr, a);
+  __syncthreads();
+  int buf = 0;
+  for (int64_t tb = from; tb < t1; tb += kScanTile, buf ^= 1) {
+    stage.fetch(a, me.group, tb + kScanTile, first_bits(t1 - tb - kScanTile));
+#pragma unroll 1
+    for (int k0 = 0; k0 < kScanTile; k0 += kAhead) {
+      const int64_t left = t1 - tb - k0;  // the tokens not done
+      if (left <= 0) break;
+      now = next;
+      px += kAhead * a.x_stride;
+      pdt += kAhead * a.dt_stride;
+      if (left >= 2 * kAhead) next.template load<false>(px, pdt, nullptr, a);
+      if (left >= kAhead) {
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (tb + k + u < t1) {
-          xr[u] = x[(uint64_t)(tb + k + u) * a.x_stride];
-          dr[u] = dt[(uint64_t)(tb + k + u) * a.dt_stride];
+        for (int j = 0; j < Batch<T, LP>::kOwn; ++j) {
+          float s = to_f32(now.dt[j]) + bias;
+          if (a.softplus) s = softplus(s);
+          sum += s;
+          const float sx = s * to_f32(now.x[j]);
+#pragma unroll
+          for (int q = 0; q < LP; ++q)
+            advance<NS, FULL>(from_lane<LP>(s, q), from_lane<LP>(sx, q), &bc[buf][k0 + j * LP + q][me.n0], a2, me.n0, N, h);
         }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        if (tb + k + u >= t1) break;
-        float s = to_f32(dr[u]) + bias;
-        if (a.softplus) s = softplus(s);
-        sum += s;
-        advance<NS, FULL>(s, s * to_f32(xr[u]), &bc[k + u][0][me.n0], a2, me.n0, N, h);
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < (int)left; ++k) {
+          const uint64_t t = (uint64_t)(tb + k0 + k);
+          float s = to_f32(dt[t * a.dt_stride]) + bias;
+          if (a.softplus) s = softplus(s);
+          if (part == 0) sum += s;
+          advance<NS, FULL>(s, s * to_f32(x[t * a.x_stride]), &bc[buf][k0 + k][me.n0], a2, me.n0, N, h);
+        }
       }
     }
+    stage.put(&bc[buf ^ 1][0][0]);
+    __syncthreads();
   }
+  sum = sum_lanes<LP>(sum);
   if (me.valid) {
-    store_states<NS, FULL>(w.state + row, me.n0, N, h);
+    store_pairs<NS, FULL>(w.state + row, me.n0, N, h);
     if (me.first) w.sum[(uint64_t)chunk * a.channels + me.c] = sum;
   }
 }
@@ -146,83 +248,137 @@ __global__ void __launch_bounds__(256) sscan_fold_kernel(const float* a, ScanWor
   }
 }
 
-// The main pass over one chunk.
-template <class T, int NS, int LP, bool FULL>
-__global__ void __launch_bounds__(kScanThreads) sscan_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
+template <int NS>
+__device__ __forceinline__ float dot(const float* c, const f32x2 (&h)[NS / 2]) {
+  f32x2 o = 0ull;
+#pragma unroll
+  for (int i = 0; i < NS / 2; i += 2) {
+    const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(c + 2 * i);
+    o = fma2(cc.x, h[i], o);
+    o = fma2(cc.y, h[i + 1], o);
+  }
+  return sum2(o);
+}
+
+// The main pass over one chunk, in batches of 8 tokens.  A batch inside one
+// sequence takes the straight path, its rows fetched while the batch before it
+// was computed; one in which a sequence begins or ends elsewhere than at its
+// edges goes token by token.
+template <class T, int NS, int LP, bool FULL, bool GATE>
+__global__ void __launch_bounds__(kScanThreads, 4) sscan_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
   constexpr int NP = NS * LP;
-  __shared__ __align__(16) float bc[kScanTile][2][NP];
+  __shared__ __align__(16) float bc[2][kScanTile][2][NP];
   const uint32_t N = a.states;
   const ScanLane<NS, LP> me(a.channels, a.groups, p.per_group, blockIdx.x % p.ctiles);
+  const uint32_t part = threadIdx.x % LP;
   const int64_t chunk = blockIdx.x / p.ctiles;
   const int64_t t0 = chunk * (int64_t)p.len, t1 = min(t0 + (int64_t)p.len, (int64_t)a.seq.tokens);
-  float h[NS], a2[NS];
-  load_states<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2);
-#pragma unroll
-  for (int j = 0; j < NS; ++j) a2[j] *= kLog2e;
-  zero_states(h);
+  f32x2 h[NS / 2], a2[NS / 2];
+  load_pairs<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2, kLog2e);
+  zero_pairs(h);
   const uint64_t row = ((uint64_t)chunk * a.channels + me.c) * N;
-  if (p.carry) load_states<NS, FULL>(w.state + row, me.n0, N, h);
+  if (p.carry) load_pairs<NS, FULL>(w.state + row, me.n0, N, h);
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
   const float dskip = a.d ? a.d[me.c] : 0.f;
   const T* x = reinterpret_cast<const T*>(a.x) + me.c;
   const T* dt = reinterpret_cast<const T*>(a.dt) + me.c;
-  const T* z = a.z ? reinterpret_cast<const T*>(a.z) + me.c : nullptr;
+  const T* z = GATE ? reinterpret_cast<const T*>(a.z) + me.c : nullptr;
   T* y = reinterpret_cast<T*>(a.y) + me.c;
 
-  for (int64_t tb = t0; tb < t1; tb += kScanTile) {
-    const TileMarks m = tile_marks(a.seq, tb, t1);
-    if (m.live == 0) continue;
-    __syncthreads();
-    stage_bc<T, NP, true>(a, me.group, tb, m.live, bc);
-    __syncthreads();
+  const auto begin_state = [&](int64_t seq) {
+    zero_pairs(h);
+    if (!a.state) return;
+    const int64_t slot = a.seq.resumes(seq) ? a.seq.slot(seq) : -1;
+    const float* from = nullptr;
+    if (w.start && p.carry && a.seq.begin(seq + 1) > t1) from = w.start + row;
+    else if (slot >= 0) from = a.state + ((uint64_t)slot * a.channels + me.c) * N;
+    if (from) load_pairs<NS, FULL>(from, me.n0, N, h);
+  };
+  const auto end_state = [&](int64_t seq) {
+    const int64_t slot = a.final_state ? a.seq.slot(seq) : -1;
+    if (slot >= 0 && me.valid)
+      store_pairs<NS, FULL>(a.final_state + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, h);
+  };
+  const auto mark = [&](int64_t t) {
+    if (a.marks && me.valid)
+      store_pairs<NS, FULL>(a.marks + ((uint64_t)(t / kMarkEvery) * a.channels + me.c) * N, me.n0, N, h);
+  };
+  const auto finish = [&](float o, float xv, float zv) {
+    o = __fmaf_rn(dskip, xv, o);
+    if (GATE) o *= zv * sigmoid(zv);
+    return from_f32<T>(o);
+  };
+  // Whether the eight tokens of these bits run straight through.
+  const auto straight = [](uint32_t live, uint32_t start, uint32_t end) {
+    return (live & 255) == 255 && !(start & 254) && !(end & 127);
+  };
+
+  StageBC<T, NP, 2> stage;
+  Batch<T, LP> now, next;
+  TileMarks m = tile_marks(a.seq, t0, t1), after;
+  stage.fetch(a, me.group, t0, m.live);
+  stage.put(&bc[0][0][0][0]);
+  const T* px = x + (uint64_t)(t0 + part) * a.x_stride;
+  const T* pdt = dt + (uint64_t)(t0 + part) * a.dt_stride;
+  const T* pz = GATE ? z + (uint64_t)(t0 + part) * a.z_stride : nullptr;
+  T* py = y + (uint64_t)(t0 + part) * a.y_stride;
+  if ((m.live & 255) == 255) next.template load<GATE>(px, pdt, pz, a);
+  __syncthreads();
+  int buf = 0;
+  for (int64_t tb = t0; tb < t1; tb += kScanTile, buf ^= 1, m = after) {
+    after = tile_marks(a.seq, tb + kScanTile, t1);
+    stage.fetch(a, me.group, tb + kScanTile, after.live);
+#pragma unroll 1
     for (int k0 = 0; k0 < kScanTile; k0 += kAhead) {
-      T xr[kAhead], dr[kAhead], zr[kAhead];
+      const uint32_t live = m.live >> k0, start = m.start >> k0, end = m.end >> k0;
+      now = next;
+      px += kAhead * a.x_stride;
+      pdt += kAhead * a.dt_stride;
+      if (GATE) pz += kAhead * a.z_stride;
+      if (((k0 + kAhead < kScanTile ? m.live >> (k0 + kAhead) : after.live) & 255) == 255) next.template load<GATE>(px, pdt, pz, a);
+      if (straight(live, start, end)) {
+        if (start & 1) begin_state(tile_seq(m, k0));
+        mark(tb + k0);
+        T* to = py;
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (m.live >> (k0 + u) & 1) {
-          const uint64_t t = (uint64_t)(tb + k0 + u);
-          xr[u] = x[t * a.x_stride];
-          dr[u] = dt[t * a.dt_stride];
-          if (z) zr[u] = z[t * a.z_stride];
-        }
+        for (int j = 0; j < Batch<T, LP>::kOwn; ++j) {
+          const float xv = to_f32(now.x[j]);
+          float s = to_f32(now.dt[j]) + bias;
+          if (a.softplus) s = softplus(s);
+          const float sx = s * xv;
+          float o[LP];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int k = k0 + u;
-        if (!(m.live >> k & 1)) continue;
-        const int64_t t = tb + k;
-        if (m.start >> k & 1) {
-          const int64_t seq = tile_seq(m, k);
-          zero_states(h);
-          if (a.state) {
-            const int64_t slot = a.seq.resumes(seq) ? a.seq.slot(seq) : -1;
-            const bool saved = w.start && p.carry && a.seq.begin(seq + 1) > t1;
-            if (saved) load_states<NS, FULL>(w.start + row, me.n0, N, h);
-            else if (slot >= 0) load_states<NS, FULL>(a.state + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, h);
+          for (int q = 0; q < LP; ++q) {
+            const float(&row)[2][NP] = bc[buf][k0 + j * LP + q];
+            advance<NS, FULL>(from_lane<LP>(s, q), from_lane<LP>(sx, q), &row[0][me.n0], a2, me.n0, N, h);
+            o[q] = dot<NS>(&row[1][me.n0], h);
           }
+          const T out = finish(scatter_sum<LP>(o, part), xv, GATE ? to_f32(now.z[j]) : 0.f);
+          if (me.valid) *to = out;
+          to += LP * a.y_stride;
         }
-        if (a.marks && t % kMarkEvery == 0 && me.valid)
-          store_states<NS, FULL>(a.marks + ((uint64_t)(t / kMarkEvery) * a.channels + me.c) * N, me.n0, N, h);
-        const float xv = to_f32(xr[u]);
-        float s = to_f32(dr[u]) + bias;
-        if (a.softplus) s = softplus(s);
-        advance<NS, FULL>(s, s * xv, &bc[k][0][me.n0], a2, me.n0, N, h);
-        float o = 0.f;
-#pragma unroll
-        for (int j = 0; j < NS; ++j) o = __fmaf_rn(bc[k][1][me.n0 + j], h[j], o);
-        o = sum_lanes<LP>(o);
-        if (a.d) o = __fmaf_rn(dskip, xv, o);
-        if (z) {
-          const float zv = to_f32(zr[u]);
-          o *= zv * sigmoid(zv);
-        }
-        if (me.valid && me.first) y[(uint64_t)t * a.y_stride] = from_f32<T>(o);
-        if ((m.end >> k & 1) && a.final_state) {
-          const int64_t slot = a.seq.slot(tile_seq(m, k));
-          if (slot >= 0 && me.valid)
-            store_states<NS, FULL>(a.final_state + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, h);
+        if (end & 128) end_state(tile_seq(m, k0 + 7));
+      } else if (live & 255) {
+#pragma unroll 1
+        for (int k = 0; k < kAhead; ++k) {
+          if (!(live >> k & 1)) continue;
+          if (start >> k & 1) begin_state(tile_seq(m, k0 + k));
+          const uint64_t t = (uint64_t)(tb + k0 + k);
+          if (k == 0) mark((int64_t)t);
+          const float xv = to_f32(x[t * a.x_stride]);
+          float s = to_f32(dt[t * a.dt_stride]) + bias;
+          if (a.softplus) s = softplus(s);
+          const float(&row)[2][NP] = bc[buf][k0 + k];
+          advance<NS, FULL>(s, s * xv, &row[0][me.n0], a2, me.n0, N, h);
+          const T out = finish(sum_lanes<LP>(dot<NS>(&row[1][me.n0], h)), xv, GATE ? to_f32(z[t * a.z_stride]) : 0.f);
+          if (me.valid && me.first) y[t * a.y_stride] = out;
+          if (end >> k & 1) end_state(tile_seq(m, k0 + k));
         }
       }
+      py += kAhead * a.y_stride;
     }
+    stage.put(&bc[buf ^ 1][0][0][0]);
+    __syncthreads();
   }
   if (!a.final_state || !me.valid) return;
   // Sequences without tokens end in the state they start from.
@@ -233,10 +389,10 @@ __global__ void __launch_bounds__(kScanThreads) sscan_kernel(SscanArgs a, ScanPl
     if (a.seq.begin(i + 1) > begin) continue;
     const int64_t slot = a.seq.slot(i);
     if (slot < 0) continue;
-    zero_states(h);
+    zero_pairs(h);
     const uint64_t at = ((uint64_t)slot * a.channels + me.c) * N;
-    if (a.state && a.seq.resumes(i)) load_states<NS, FULL>(a.state + at, me.n0, N, h);
-    store_states<NS, FULL>(a.final_state + at, me.n0, N, h);
+    if (a.state && a.seq.resumes(i)) load_pairs<NS, FULL>(a.state + at, me.n0, N, h);
+    store_pairs<NS, FULL>(a.final_state + at, me.n0, N, h);
   }
 }
 
@@ -282,18 +438,19 @@ __global__ void __launch_bounds__(kScanThreads) sscan_step_kernel(SscanArgs a, u
 
 bool aligned16(const void* p) { return reinterpret_cast<uint64_t>(p) % 16 == 0; }
 
-// The states a lane holds: 16, or 8 where there are no more.
-constexpr uint32_t lanes_of(uint32_t states) { return states <= 16 ? 1 : states <= 32 ? 2 : 4; }
-constexpr uint32_t kWantedBlocks = kSms * 4;
+// The lanes that share a channel: at most 16 states each; at least 4.
+constexpr uint32_t padded(uint32_t states) { return states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
+ScanLanes lanes_of(uint32_t states) {
+  const uint32_t np = padded(states);
+  return {np <= 16 ? 1u : np / 16, np <= 8 ? 2u : np <= 32 ? 4u : 8u};
+}
 
 ScanPlan plan_of(const SscanArgs& a) {
-  return scan_plan(a.seq.tokens, a.channels, a.groups, a.seq.n_seq, a.seq.seq_ptr != nullptr,
-                   kScanThreads / lanes_of(a.states), kWantedBlocks);
+  return scan_plan(a.seq.tokens, a.channels, a.groups, a.seq.n_seq, a.seq.seq_ptr != nullptr, lanes_of(a.states));
 }
 
 template <class T, int NS, int LP, bool FULL>
-cudaError_t go(const SscanArgs& a, cudaStream_t s) {
-  const ScanPlan p = plan_of(a);
+cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
   ScanWork w{};
   scan_work(p, a.channels, a.states, true, a.work, &w);
   if (a.state != a.final_state || !a.state) w.start = nullptr;
@@ -304,7 +461,8 @@ cudaError_t go(const SscanArgs& a, cudaStream_t s) {
     const uint64_t cells = (uint64_t)a.channels * a.states;
     sscan_fold_kernel<false><<<(unsigned)((cells + 255) / 256), 256, 0, s>>>(a.a, w, p.chunks, a.channels, a.states);
   }
-  sscan_kernel<T, NS, LP, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w);
+  if (a.z) sscan_kernel<T, NS, LP, FULL, true><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w);
+  else sscan_kernel<T, NS, LP, FULL, false><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w);
   return cudaGetLastError();
 }
 
@@ -317,18 +475,32 @@ cudaError_t go_step(const SscanArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+template <class T, int NP, bool FULL>
+cudaError_t by_lanes(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
+  if constexpr (NP <= 16)
+    if (p.lanes == 1) return go<T, NP, 1, FULL>(a, p, s);
+  if constexpr (NP <= 32)
+    if (p.lanes == 2) return go<T, NP / 2, 2, FULL>(a, p, s);
+  if constexpr (NP >= 16)
+    if (p.lanes == 4) return go<T, NP / 4, 4, FULL>(a, p, s);
+  if constexpr (NP == 64)
+    if (p.lanes == 8) return go<T, NP / 8, 8, FULL>(a, p, s);
+  return cudaErrorInvalidValue;
+}
+
 template <class T>
 cudaError_t by_states(const SscanArgs& a, cudaStream_t s) {
   const uint32_t N = a.states;
+  const ScanPlan p = plan_of(a);
   const bool al = aligned16(a.a) && aligned16(a.state) && aligned16(a.final_state) && aligned16(a.marks) && aligned16(a.work);
-  if (N == 16 && al) return go<T, 16, 1, true>(a, s);
-  if (N == 8 && al) return go<T, 8, 1, true>(a, s);
-  if (N == 32 && al) return go<T, 16, 2, true>(a, s);
-  if (N == 64 && al) return go<T, 16, 4, true>(a, s);
-  if (N <= 8) return go<T, 8, 1, false>(a, s);
-  if (N <= 16) return go<T, 16, 1, false>(a, s);
-  if (N <= 32) return go<T, 16, 2, false>(a, s);
-  return go<T, 16, 4, false>(a, s);
+  if (N == 16 && al) return by_lanes<T, 16, true>(a, p, s);
+  if (N == 8 && al) return by_lanes<T, 8, true>(a, p, s);
+  if (N == 32 && al) return by_lanes<T, 32, true>(a, p, s);
+  if (N == 64 && al) return by_lanes<T, 64, true>(a, p, s);
+  if (N <= 8) return by_lanes<T, 8, false>(a, p, s);
+  if (N <= 16) return by_lanes<T, 16, false>(a, p, s);
+  if (N <= 32) return by_lanes<T, 32, false>(a, p, s);
+  return by_lanes<T, 64, false>(a, p, s);
 }
 
 template <class T>
@@ -351,7 +523,7 @@ cudaError_t step_by_states(const SscanArgs& a, cudaStream_t s) {
 size_t sscan_bytes(uint64_t tokens, uint64_t channels, uint32_t states, uint64_t n_seq, uint32_t groups) {
   uint64_t most = 0;
   for (bool ragged : {false, true}) {
-    const ScanPlan p = scan_plan(tokens, (uint32_t)channels, groups, n_seq, ragged, kScanThreads / lanes_of(states), kWantedBlocks);
+    const ScanPlan p = scan_plan(tokens, (uint32_t)channels, groups, n_seq, ragged, lanes_of(states));
     if (!p.carry) continue;
     const uint64_t b = scan_work(p, (uint32_t)channels, states, true, nullptr, nullptr);
     if (b > most) most = b;

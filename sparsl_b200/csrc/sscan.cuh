@@ -11,6 +11,7 @@ constexpr uint32_t kMarkEvery = 8;  // tokens between two saved states of a trai
 constexpr int kScanThreads = 128;
 constexpr int kScanTile = 32;       // tokens whose B and C are staged at a time
 constexpr uint32_t kSms = 148;
+constexpr uint32_t kScanBlocks = 4 * kSms;  // resident at 128 registers a thread
 
 // The token axis [0, tokens) in chunks of `len` tokens (a multiple of 32),
 // whatever sequences they hold.  `carry`: a sequence may span chunks, so the
@@ -18,40 +19,47 @@ constexpr uint32_t kSms = 148;
 struct ScanPlan {
   uint32_t ctiles;     // channel tiles, each within one group
   uint32_t per_group;  // of which each group has this many
+  uint32_t lanes;      // that share a channel
   uint64_t len, chunks;
   bool carry;
 };
 
-// `wanted` blocks fill the GPU: where the channel tiles and the sequences are
-// fewer, the token axis is split, which costs the exponentials of the spanning
-// sequences once more (for the states at the chunks' starts).
-inline ScanPlan scan_plan(uint64_t tokens, uint32_t channels, uint32_t groups, uint64_t n_seq, bool ragged,
-                          uint32_t tile_channels, uint32_t wanted) {
+// How many lanes share a channel's states: `least` is what the registers
+// demand, up to `most`.
+struct ScanLanes {
+  uint32_t least, most;
+};
+
+inline ScanPlan scan_plan(uint64_t tokens, uint32_t channels, uint32_t groups, uint64_t n_seq, bool ragged, ScanLanes l) {
   ScanPlan p;
   const uint32_t cpg = channels / groups;
-  p.per_group = (cpg + tile_channels - 1) / tile_channels;
-  p.ctiles = p.per_group * groups;
+  const auto tiles = [&](uint32_t lanes) { return (cpg + kScanThreads / lanes - 1) / (kScanThreads / lanes); };
   const uint64_t run = n_seq ? tokens / n_seq : 0;
-  const uint64_t want = (wanted + p.ctiles - 1) / p.ctiles;
-  uint64_t len = (tokens + want - 1) / want;
-  len = len < 64 ? 64 : (len + 31) / 32 * 32;
-  bool whole = false;  // no sequence spans two chunks
-  if (!ragged && run && run % 32 == 0) {
-    if (n_seq >= want || run <= 64) {
-      len = run;
-      whole = true;
-    } else {
-      // A chunk length that divides the runs, if one of at least half the size does.
-      for (uint64_t l = len; 2 * l >= len && l >= 32; l -= 32)
-        if (run % l == 0) {
-          len = l;
-          break;
-        }
+  // Whole sequences, one pass: where they and the channels give each SM three
+  // blocks or more, by as few lanes a channel as do.
+  p.lanes = 0;
+  if (!ragged && run && run % 32 == 0)
+    for (uint32_t k = l.least; k <= l.most && !p.lanes; k *= 2)
+      if (n_seq * groups * tiles(k) >= 3 * kSms || run <= 64) p.lanes = k;
+  if (p.lanes) {
+    p.len = run;
+    p.chunks = n_seq;
+    p.carry = false;
+  } else {
+    // One wave of blocks over equal chunks, of 64 tokens at least; more lanes a
+    // channel where that leaves SMs with fewer than three blocks.
+    for (uint32_t k = l.least; k <= l.most; k *= 2) {
+      const uint64_t ct = (uint64_t)groups * tiles(k), want = ct >= kScanBlocks ? 1 : kScanBlocks / ct;
+      p.lanes = k;
+      p.len = (tokens + want - 1) / want;
+      p.len = p.len < 64 ? 64 : (p.len + 31) / 32 * 32;
+      p.chunks = tokens ? (tokens + p.len - 1) / p.len : 1;
+      if (p.chunks * ct >= 3 * kSms) break;
     }
+    p.carry = p.chunks > 1;
   }
-  p.len = len;
-  p.chunks = tokens ? (tokens + len - 1) / len : 1;
-  p.carry = !whole && p.chunks > 1;
+  p.per_group = tiles(p.lanes);
+  p.ctiles = p.per_group * groups;
   return p;
 }
 

@@ -24,7 +24,6 @@ cudaError_t launch_sscan_fold_back(const float* a, const ScanWork& w, uint64_t c
 namespace {
 
 constexpr int kWarps = kScanThreads / 32;
-constexpr uint32_t kWantedBlocks = kSms * 4;
 
 struct BackWork {
   ScanWork scan;
@@ -371,7 +370,7 @@ bool aligned16(const void* p) { return reinterpret_cast<uint64_t>(p) % 16 == 0; 
 constexpr uint32_t lanes_of(uint32_t states) { return states <= 8 ? 1 : states <= 16 ? 2 : states <= 32 ? 4 : 8; }
 
 ScanPlan plan_of(uint64_t tokens, uint32_t channels, uint32_t states, uint64_t n_seq, uint32_t groups, bool ragged) {
-  return scan_plan(tokens, channels, groups, n_seq, ragged, kScanThreads / lanes_of(states), kWantedBlocks);
+  return scan_plan(tokens, channels, groups, n_seq, ragged, {lanes_of(states), lanes_of(states)});
 }
 
 uint64_t back_work(const ScanPlan& p, uint64_t tokens, uint32_t channels, uint32_t states, uint32_t groups, void* base,
