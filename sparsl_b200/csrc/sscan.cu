@@ -18,12 +18,13 @@ namespace sparsl {
 namespace {
 
 constexpr int kAhead = 8;  // tokens in a batch: the next batch's rows are loaded while one is computed
+constexpr uint32_t kResident = 4;  // blocks an SM holds, at 128 registers a thread
 
-// One token of NS states, two at a time: h <- e h + (s x) B.
+// One token: h <- e h + (s x) B.
 template <int NS, bool FULL>
-__device__ __forceinline__ void advance(float s, float sx, const float* b, const f32x2 (&a2)[NS / 2], uint32_t n0, uint32_t N,
+__device__ __forceinline__ void advance(const f32x2 (&e)[NS / 2], float sx, const float* b, uint32_t n0, uint32_t N,
                                         f32x2 (&h)[NS / 2]) {
-  const f32x2 ss = pair(s, s), xx = pair(sx, sx);
+  const f32x2 xx = pair(sx, sx);
 #pragma unroll
   for (int j = 0; j < NS / 2; j += 2) {
     const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(b + 2 * j);
@@ -35,59 +36,10 @@ __device__ __forceinline__ void advance(float s, float sx, const float* b, const
       unpair(add1, lo, hi);
       add1 = pair(n0 + 2 * j + 2 < N ? lo : 0.f, n0 + 2 * j + 3 < N ? hi : 0.f);
     }
-    h[j] = fma2(ex2_2(mul2(ss, a2[j])), h[j], add0);
-    h[j + 1] = fma2(ex2_2(mul2(ss, a2[j + 1])), h[j + 1], add1);
+    h[j] = fma2(e[j], h[j], add0);
+    h[j + 1] = fma2(e[j + 1], h[j + 1], add1);
   }
 }
-
-template <int NS, bool FULL>
-__device__ __forceinline__ void load_pairs(const float* p, uint32_t n0, uint32_t N, f32x2 (&h)[NS / 2], float scale = 1.f) {
-  float v[NS];
-  load_states<NS, FULL>(p, n0, N, v);
-#pragma unroll
-  for (int j = 0; j < NS / 2; ++j) h[j] = pair(v[2 * j] * scale, v[2 * j + 1] * scale);
-}
-template <int NS, bool FULL>
-__device__ __forceinline__ void store_pairs(float* p, uint32_t n0, uint32_t N, const f32x2 (&h)[NS / 2]) {
-  float v[NS];
-#pragma unroll
-  for (int j = 0; j < NS / 2; ++j) unpair(h[j], v[2 * j], v[2 * j + 1]);
-  store_states<NS, FULL>(p, n0, N, v);
-}
-template <int M>
-__device__ __forceinline__ void zero_pairs(f32x2 (&h)[M]) {
-#pragma unroll
-  for (int j = 0; j < M; ++j) h[j] = 0ull;
-}
-
-// The rows of B, and behind each those of C (R = 2), of a tile's tokens: every
-// thread fetches some values of the next tile while one is computed, and puts
-// them, as f32, into the other of two buffers.
-template <class T, int NP, int R>
-struct StageBC {
-  static constexpr int kEach = (kScanTile * R * NP + kScanThreads - 1) / kScanThreads;
-  T v[kEach];
-  uint32_t got;
-  __device__ __forceinline__ void fetch(const SscanArgs& a, uint32_t group, int64_t tb, uint32_t live) {
-    got = 0;
-#pragma unroll
-    for (int q = 0; q < kEach; ++q) {
-      const uint32_t i = q * kScanThreads + threadIdx.x, n = i % NP, which = i / NP % R, k = i / (NP * R);
-      if (k < (uint32_t)kScanTile && (live >> k & 1) && n < a.states) {
-        const T* p = reinterpret_cast<const T*>(which ? a.c : a.b);
-        v[q] = p[(uint64_t)(tb + k) * (which ? a.c_stride : a.b_stride) + (uint64_t)group * (which ? a.c_group : a.b_group) + n];
-        got |= 1u << q;
-      }
-    }
-  }
-  __device__ __forceinline__ void put(float* sh) const {
-#pragma unroll
-    for (int q = 0; q < kEach; ++q) {
-      const uint32_t i = q * kScanThreads + threadIdx.x;
-      if (i < kScanTile * R * NP) sh[i] = got >> q & 1 ? to_f32(v[q]) : 0.f;
-    }
-  }
-};
 
 // Rows of a batch, one token in LP of them per lane: the lanes that share a
 // channel divide a token's own work (step, gate, output) among them.
@@ -111,32 +63,10 @@ struct Batch {
   }
 };
 
-template <int LP>
-__device__ __forceinline__ float from_lane(float v, int q) {
-  if constexpr (LP == 1) return v;
-  else return __shfl_sync(0xffffffffu, v, q, LP);
-}
-// o[q] of LP lanes: lane q gets the sum of their o[q].
-template <int LP>
-__device__ __forceinline__ float scatter_sum(float (&o)[LP], uint32_t part) {
-#pragma unroll
-  for (int w = LP / 2; w >= 1; w /= 2) {
-    const bool up = part & w;
-#pragma unroll
-    for (int j = 0; j < w; ++j) {
-      const float send = up ? o[j] : o[j + w], keep = up ? o[j + w] : o[j];
-      o[j] = keep + __shfl_xor_sync(0xffffffffu, send, w);
-    }
-  }
-  return o[0];
-}
-
-__device__ __forceinline__ uint32_t first_bits(int64_t n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
-
 // The state that a chunk hands to the next one: its last sequence's, from that
 // sequence's start in it or from zero.
 template <class T, int NS, int LP, bool FULL>
-__global__ void __launch_bounds__(kScanThreads, 4) sscan_chunk_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
+__global__ void __launch_bounds__(kScanThreads, kResident) sscan_chunk_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
   constexpr int NP = NS * LP;
   __shared__ __align__(16) float bc[2][kScanTile][NP];
   const uint32_t N = a.states;
@@ -184,15 +114,22 @@ __global__ void __launch_bounds__(kScanThreads, 4) sscan_chunk_kernel(SscanArgs 
       pdt += kAhead * a.dt_stride;
       if (left >= 2 * kAhead) next.template load<false>(px, pdt, nullptr, a);
       if (left >= kAhead) {
+        float s[Batch<T, LP>::kOwn], sx[Batch<T, LP>::kOwn];
 #pragma unroll
         for (int j = 0; j < Batch<T, LP>::kOwn; ++j) {
-          float s = to_f32(now.dt[j]) + bias;
-          if (a.softplus) s = softplus(s);
-          sum += s;
-          const float sx = s * to_f32(now.x[j]);
+          s[j] = to_f32(now.dt[j]) + bias;
+          if (a.softplus) s[j] = softplus(s[j]);
+          sum += s[j];
+          sx[j] = s[j] * to_f32(now.x[j]);
+        }
+        f32x2 e[NS / 2], en[NS / 2];
+        decay<NS>(from_lane<LP>(s[0], 0), a2, e);
 #pragma unroll
-          for (int q = 0; q < LP; ++q)
-            advance<NS, FULL>(from_lane<LP>(s, q), from_lane<LP>(sx, q), &bc[buf][k0 + j * LP + q][me.n0], a2, me.n0, N, h);
+        for (int k = 0; k < kAhead; ++k) {  // a token's exponentials are under way while the one before it is added
+          if (k + 1 < kAhead) decay<NS>(from_lane<LP>(s[(k + 1) / LP], (k + 1) % LP), a2, en);
+          advance<NS, FULL>(e, from_lane<LP>(sx[k / LP], k % LP), &bc[buf][k0 + k][me.n0], me.n0, N, h);
+#pragma unroll
+          for (int i = 0; i < NS / 2; ++i) e[i] = en[i];
         }
       } else {
 #pragma unroll 1
@@ -201,7 +138,9 @@ __global__ void __launch_bounds__(kScanThreads, 4) sscan_chunk_kernel(SscanArgs 
           float s = to_f32(dt[t * a.dt_stride]) + bias;
           if (a.softplus) s = softplus(s);
           if (part == 0) sum += s;
-          advance<NS, FULL>(s, s * to_f32(x[t * a.x_stride]), &bc[buf][k0 + k][me.n0], a2, me.n0, N, h);
+          f32x2 e[NS / 2];
+          decay<NS>(s, a2, e);
+          advance<NS, FULL>(e, s * to_f32(x[t * a.x_stride]), &bc[buf][k0 + k][me.n0], me.n0, N, h);
         }
       }
     }
@@ -250,22 +189,22 @@ __global__ void __launch_bounds__(256) sscan_fold_kernel(const float* a, ScanWor
 
 template <int NS>
 __device__ __forceinline__ float dot(const float* c, const f32x2 (&h)[NS / 2]) {
-  f32x2 o = 0ull;
+  f32x2 o = 0ull, p = 0ull;
 #pragma unroll
   for (int i = 0; i < NS / 2; i += 2) {
     const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(c + 2 * i);
     o = fma2(cc.x, h[i], o);
-    o = fma2(cc.y, h[i + 1], o);
+    p = fma2(cc.y, h[i + 1], p);
   }
-  return sum2(o);
+  return sum2(add2(o, p));
 }
 
-// The main pass over one chunk, in batches of 8 tokens.  A batch inside one
+// The main pass over one chunk, in batches of kAhead tokens.  A batch inside one
 // sequence takes the straight path, its rows fetched while the batch before it
 // was computed; one in which a sequence begins or ends elsewhere than at its
 // edges goes token by token.
 template <class T, int NS, int LP, bool FULL, bool GATE>
-__global__ void __launch_bounds__(kScanThreads, 4) sscan_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
+__global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
   constexpr int NP = NS * LP;
   __shared__ __align__(16) float bc[2][kScanTile][2][NP];
   const uint32_t N = a.states;
@@ -300,7 +239,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) sscan_kernel(SscanArgs a, Sca
       store_pairs<NS, FULL>(a.final_state + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, h);
   };
   const auto mark = [&](int64_t t) {
-    if (a.marks && me.valid)
+    if (a.marks && t % kMarkEvery == 0 && me.valid)
       store_pairs<NS, FULL>(a.marks + ((uint64_t)(t / kMarkEvery) * a.channels + me.c) * N, me.n0, N, h);
   };
   const auto finish = [&](float o, float xv, float zv) {
@@ -308,9 +247,10 @@ __global__ void __launch_bounds__(kScanThreads, 4) sscan_kernel(SscanArgs a, Sca
     if (GATE) o *= zv * sigmoid(zv);
     return from_f32<T>(o);
   };
-  // Whether the eight tokens of these bits run straight through.
+  // Whether the tokens of a batch run straight through.
+  constexpr uint32_t kFull = (1u << kAhead) - 1;
   const auto straight = [](uint32_t live, uint32_t start, uint32_t end) {
-    return (live & 255) == 255 && !(start & 254) && !(end & 127);
+    return (live & kFull) == kFull && !(start & kFull & ~1u) && !(end & (kFull >> 1));
   };
 
   StageBC<T, NP, 2> stage;
@@ -322,7 +262,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) sscan_kernel(SscanArgs a, Sca
   const T* pdt = dt + (uint64_t)(t0 + part) * a.dt_stride;
   const T* pz = GATE ? z + (uint64_t)(t0 + part) * a.z_stride : nullptr;
   T* py = y + (uint64_t)(t0 + part) * a.y_stride;
-  if ((m.live & 255) == 255) next.template load<GATE>(px, pdt, pz, a);
+  if ((m.live & kFull) == kFull) next.template load<GATE>(px, pdt, pz, a);
   __syncthreads();
   int buf = 0;
   for (int64_t tb = t0; tb < t1; tb += kScanTile, buf ^= 1, m = after) {
@@ -335,41 +275,51 @@ __global__ void __launch_bounds__(kScanThreads, 4) sscan_kernel(SscanArgs a, Sca
       px += kAhead * a.x_stride;
       pdt += kAhead * a.dt_stride;
       if (GATE) pz += kAhead * a.z_stride;
-      if (((k0 + kAhead < kScanTile ? m.live >> (k0 + kAhead) : after.live) & 255) == 255) next.template load<GATE>(px, pdt, pz, a);
+      if (((k0 + kAhead < kScanTile ? m.live >> (k0 + kAhead) : after.live) & kFull) == kFull) next.template load<GATE>(px, pdt, pz, a);
       if (straight(live, start, end)) {
         if (start & 1) begin_state(tile_seq(m, k0));
         mark(tb + k0);
         T* to = py;
+        float s[Batch<T, LP>::kOwn], sx[Batch<T, LP>::kOwn], xv[Batch<T, LP>::kOwn], o[LP];
 #pragma unroll
         for (int j = 0; j < Batch<T, LP>::kOwn; ++j) {
-          const float xv = to_f32(now.x[j]);
-          float s = to_f32(now.dt[j]) + bias;
-          if (a.softplus) s = softplus(s);
-          const float sx = s * xv;
-          float o[LP];
-#pragma unroll
-          for (int q = 0; q < LP; ++q) {
-            const float(&row)[2][NP] = bc[buf][k0 + j * LP + q];
-            advance<NS, FULL>(from_lane<LP>(s, q), from_lane<LP>(sx, q), &row[0][me.n0], a2, me.n0, N, h);
-            o[q] = dot<NS>(&row[1][me.n0], h);
-          }
-          const T out = finish(scatter_sum<LP>(o, part), xv, GATE ? to_f32(now.z[j]) : 0.f);
-          if (me.valid) *to = out;
-          to += LP * a.y_stride;
+          xv[j] = to_f32(now.x[j]);
+          s[j] = to_f32(now.dt[j]) + bias;
+          if (a.softplus) s[j] = softplus(s[j]);
+          sx[j] = s[j] * xv[j];
         }
-        if (end & 128) end_state(tile_seq(m, k0 + 7));
-      } else if (live & 255) {
+        f32x2 e[NS / 2], en[NS / 2];
+        decay<NS>(from_lane<LP>(s[0], 0), a2, e);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {  // a token's exponentials are under way while the one before it is added
+          const int j = k / LP, q = k % LP;
+          if (k + 1 < kAhead) decay<NS>(from_lane<LP>(s[(k + 1) / LP], (k + 1) % LP), a2, en);
+          const float(&row)[2][NP] = bc[buf][k0 + k];
+          advance<NS, FULL>(e, from_lane<LP>(sx[j], q), &row[0][me.n0], me.n0, N, h);
+          o[q] = dot<NS>(&row[1][me.n0], h);
+          if (q == LP - 1) {
+            const T out = finish(scatter_sum<LP>(o, part), xv[j], GATE ? to_f32(now.z[j]) : 0.f);
+            if (me.valid) *to = out;
+            to += LP * a.y_stride;
+          }
+#pragma unroll
+          for (int i = 0; i < NS / 2; ++i) e[i] = en[i];
+        }
+        if (end >> (kAhead - 1) & 1) end_state(tile_seq(m, k0 + kAhead - 1));
+      } else if (live & kFull) {
 #pragma unroll 1
         for (int k = 0; k < kAhead; ++k) {
           if (!(live >> k & 1)) continue;
           if (start >> k & 1) begin_state(tile_seq(m, k0 + k));
           const uint64_t t = (uint64_t)(tb + k0 + k);
-          if (k == 0) mark((int64_t)t);
+          mark((int64_t)t);
           const float xv = to_f32(x[t * a.x_stride]);
           float s = to_f32(dt[t * a.dt_stride]) + bias;
           if (a.softplus) s = softplus(s);
           const float(&row)[2][NP] = bc[buf][k0 + k];
-          advance<NS, FULL>(s, s * xv, &row[0][me.n0], a2, me.n0, N, h);
+          f32x2 e[NS / 2];
+          decay<NS>(s, a2, e);
+          advance<NS, FULL>(e, s * xv, &row[0][me.n0], me.n0, N, h);
           const T out = finish(sum_lanes<LP>(dot<NS>(&row[1][me.n0], h)), xv, GATE ? to_f32(z[t * a.z_stride]) : 0.f);
           if (me.valid && me.first) y[t * a.y_stride] = out;
           if (end >> k & 1) end_state(tile_seq(m, k0 + k));
@@ -442,7 +392,7 @@ bool aligned16(const void* p) { return reinterpret_cast<uint64_t>(p) % 16 == 0; 
 constexpr uint32_t padded(uint32_t states) { return states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
 ScanLanes lanes_of(uint32_t states) {
   const uint32_t np = padded(states);
-  return {np <= 16 ? 1u : np / 16, np <= 8 ? 2u : np <= 32 ? 4u : 8u};
+  return {np <= 16 ? 1u : np / 16, np <= 8 ? 2u : 4u, kResident};
 }
 
 ScanPlan plan_of(const SscanArgs& a) {
@@ -483,8 +433,6 @@ cudaError_t by_lanes(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
     if (p.lanes == 2) return go<T, NP / 2, 2, FULL>(a, p, s);
   if constexpr (NP >= 16)
     if (p.lanes == 4) return go<T, NP / 4, 4, FULL>(a, p, s);
-  if constexpr (NP == 64)
-    if (p.lanes == 8) return go<T, NP / 8, 8, FULL>(a, p, s);
   return cudaErrorInvalidValue;
 }
 

@@ -11,7 +11,6 @@ constexpr uint32_t kMarkEvery = 8;  // tokens between two saved states of a trai
 constexpr int kScanThreads = 128;
 constexpr int kScanTile = 32;       // tokens whose B and C are staged at a time
 constexpr uint32_t kSms = 148;
-constexpr uint32_t kScanBlocks = 4 * kSms;  // resident at 128 registers a thread
 
 // The token axis [0, tokens) in chunks of `len` tokens (a multiple of 32),
 // whatever sequences they hold.  `carry`: a sequence may span chunks, so the
@@ -25,39 +24,39 @@ struct ScanPlan {
 };
 
 // How many lanes share a channel's states: `least` is what the registers
-// demand, up to `most`.
+// demand, up to `most`; and the blocks that an SM holds.
 struct ScanLanes {
-  uint32_t least, most;
+  uint32_t least, most, resident;
 };
 
 inline ScanPlan scan_plan(uint64_t tokens, uint32_t channels, uint32_t groups, uint64_t n_seq, bool ragged, ScanLanes l) {
   ScanPlan p;
   const uint32_t cpg = channels / groups;
   const auto tiles = [&](uint32_t lanes) { return (cpg + kScanThreads / lanes - 1) / (kScanThreads / lanes); };
-  const uint64_t run = n_seq ? tokens / n_seq : 0;
-  // Whole sequences, one pass: where they and the channels give each SM three
-  // blocks or more, by as few lanes a channel as do.
-  p.lanes = 0;
-  if (!ragged && run && run % 32 == 0)
-    for (uint32_t k = l.least; k <= l.most && !p.lanes; k *= 2)
-      if (n_seq * groups * tiles(k) >= 3 * kSms || run <= 64) p.lanes = k;
-  if (p.lanes) {
-    p.len = run;
-    p.chunks = n_seq;
-    p.carry = false;
-  } else {
-    // One wave of blocks over equal chunks, of 64 tokens at least; more lanes a
-    // channel where that leaves SMs with fewer than three blocks.
-    for (uint32_t k = l.least; k <= l.most; k *= 2) {
-      const uint64_t ct = (uint64_t)groups * tiles(k), want = ct >= kScanBlocks ? 1 : kScanBlocks / ct;
-      p.lanes = k;
-      p.len = (tokens + want - 1) / want;
-      p.len = p.len < 64 ? 64 : (p.len + 31) / 32 * 32;
-      p.chunks = tokens ? (tokens + p.len - 1) / p.len : 1;
-      if (p.chunks * ct >= 3 * kSms) break;
-    }
-    p.carry = p.chunks > 1;
+  const uint64_t run = n_seq ? tokens / n_seq : 0, slots = (uint64_t)kSms * l.resident;
+  // One wave of blocks over equal chunks, of 64 tokens at least; more lanes a
+  // channel where that leaves SMs with fewer than three quarters of their blocks.
+  for (uint32_t k = l.least; k <= l.most; k *= 2) {
+    const uint64_t ct = (uint64_t)groups * tiles(k), want = ct >= slots ? 1 : slots / ct;
+    p.lanes = k;
+    p.len = (tokens + want - 1) / want;
+    p.len = p.len < 64 ? 64 : (p.len + 31) / 32 * 32;
+    p.chunks = tokens ? (tokens + p.len - 1) / p.len : 1;
+    if (4 * p.chunks * ct >= 3 * slots) break;
   }
+  p.carry = p.chunks > 1;
+  // Whole sequences instead, in one pass without the states at the chunks'
+  // starts, where they fill at least three quarters of their waves of blocks.
+  if (!ragged && run && run % 32 == 0)
+    for (uint32_t k = l.least; k <= l.most; k *= 2) {
+      const uint64_t blocks = n_seq * groups * tiles(k), waves = (blocks + slots - 1) / slots;
+      if (4 * blocks < 3 * waves * slots && run > 64) continue;
+      p.lanes = k;
+      p.len = run;
+      p.chunks = n_seq;
+      p.carry = false;
+      break;
+    }
   p.per_group = tiles(p.lanes);
   p.ctiles = p.per_group * groups;
   return p;
@@ -196,5 +195,84 @@ __device__ __forceinline__ float sum_lanes(float v) {
   for (int o = 1; o < LP; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+
+// The decays exp(s A) of NS states, two at a time.
+template <int NS>
+__device__ __forceinline__ void decay(float s, const f32x2 (&a2)[NS / 2], f32x2 (&e)[NS / 2]) {
+  const f32x2 ss = pair(s, s);
+#pragma unroll
+  for (int j = 0; j < NS / 2; ++j) e[j] = ex2_2(mul2(ss, a2[j]));
+}
+template <int NS, bool FULL>
+__device__ __forceinline__ void load_pairs(const float* p, uint32_t n0, uint32_t N, f32x2 (&h)[NS / 2], float scale = 1.f) {
+  float v[NS];
+  load_states<NS, FULL>(p, n0, N, v);
+#pragma unroll
+  for (int j = 0; j < NS / 2; ++j) h[j] = pair(v[2 * j] * scale, v[2 * j + 1] * scale);
+}
+template <int NS, bool FULL>
+__device__ __forceinline__ void store_pairs(float* p, uint32_t n0, uint32_t N, const f32x2 (&h)[NS / 2]) {
+  float v[NS];
+#pragma unroll
+  for (int j = 0; j < NS / 2; ++j) unpair(h[j], v[2 * j], v[2 * j + 1]);
+  store_states<NS, FULL>(p, n0, N, v);
+}
+template <int M>
+__device__ __forceinline__ void zero_pairs(f32x2 (&h)[M]) {
+#pragma unroll
+  for (int j = 0; j < M; ++j) h[j] = 0ull;
+}
+
+// The rows of B, and behind each those of C (R = 2; FROM_C: of C alone), of a tile's tokens: every
+// thread fetches some values of the next tile while one is computed, and puts
+// them, as f32, into the other of two buffers.
+template <class T, int NP, int R, bool FROM_C = false>
+struct StageBC {
+  static constexpr int kEach = (kScanTile * R * NP + kScanThreads - 1) / kScanThreads;
+  T v[kEach];
+  uint32_t got;
+  __device__ __forceinline__ void fetch(const SscanArgs& a, uint32_t group, int64_t tb, uint32_t live) {
+    got = 0;
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      const uint32_t i = q * kScanThreads + threadIdx.x, n = i % NP, which = i / NP % R, k = i / (NP * R);
+      if (k < (uint32_t)kScanTile && (live >> k & 1) && n < a.states) {
+        const bool c = FROM_C || which;
+        const T* p = reinterpret_cast<const T*>(c ? a.c : a.b);
+        v[q] = p[(uint64_t)(tb + k) * (c ? a.c_stride : a.b_stride) + (uint64_t)group * (c ? a.c_group : a.b_group) + n];
+        got |= 1u << q;
+      }
+    }
+  }
+  __device__ __forceinline__ void put(float* sh) const {
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) {
+      const uint32_t i = q * kScanThreads + threadIdx.x;
+      if (i < kScanTile * R * NP) sh[i] = got >> q & 1 ? to_f32(v[q]) : 0.f;
+    }
+  }
+};
+
+template <int LP>
+__device__ __forceinline__ float from_lane(float v, int q) {
+  if constexpr (LP == 1) return v;
+  else return __shfl_sync(0xffffffffu, v, q, LP);
+}
+// o[q] of LP lanes: lane q gets the sum of their o[q].
+template <int LP>
+__device__ __forceinline__ float scatter_sum(float (&o)[LP], uint32_t part) {
+#pragma unroll
+  for (int w = LP / 2; w >= 1; w /= 2) {
+    const bool up = part & w;
+#pragma unroll
+    for (int j = 0; j < w; ++j) {
+      const float send = up ? o[j] : o[j + w], keep = up ? o[j + w] : o[j];
+      o[j] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+    }
+  }
+  return o[0];
+}
+
+__device__ __forceinline__ uint32_t first_bits(int64_t n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
 
 }  // namespace sparsl

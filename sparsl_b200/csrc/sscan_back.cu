@@ -10,10 +10,10 @@
 // states kept in registers, and then walked backwards, so each exponential is
 // computed once.  Chunks of the token axis run in parallel as in the forward
 // pass: the gradient each chunk hands to the one before it is computed first,
-// and folded.  dB and dC are summed over a warp's channels by exchanges that
-// halve what a lane holds, over a block's warps in shared memory, and over the
-// blocks' partial rows in a fixed order, so that results do not change from run
-// to run; so are dA, dD and the step bias's gradient over the chunks.
+// and folded.  dB and dC are summed over a warp's channels and a block's warps
+// in shared memory, and over the blocks' partial rows in a fixed order, so that
+// results do not change from run to run; so are dA, dD and the step bias's
+// gradient over the chunks.
 #include "sscan.cuh"
 
 namespace sparsl {
@@ -24,6 +24,8 @@ cudaError_t launch_sscan_fold_back(const float* a, const ScanWork& w, uint64_t c
 namespace {
 
 constexpr int kWarps = kScanThreads / 32;
+constexpr uint32_t kResident = 2;  // blocks an SM holds, at up to 255 registers a thread
+constexpr int kBlock = (int)kMarkEvery;
 
 struct BackWork {
   ScanWork scan;
@@ -35,14 +37,15 @@ struct BackWork {
 __device__ __forceinline__ float gate_grad(float z, float sig) { return sig * __fmaf_rn(z, 1.0f - sig, 1.0f); }
 
 // The gradient that a chunk hands to the state before it, from the end of the
-// sequence that reaches into it, or from zero at its own end.
-template <class T, int NS, int LP, bool FULL>
-__global__ void __launch_bounds__(kScanThreads) sscan_chunk_back_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
-  constexpr int NP = NS * LP;
-  constexpr int U = 8;
-  __shared__ __align__(16) float sc[kScanTile][NP];
+// sequence that reaches into it, or from zero at its own end; in batches of
+// eight tokens, the last ones first.
+template <class T, int NS, int LP, bool FULL, bool GATE>
+__global__ void __launch_bounds__(kScanThreads, 4) sscan_chunk_back_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
+  constexpr int NP = NS * LP, U = 8, kOwn = U / LP;
+  __shared__ __align__(16) float sc[2][kScanTile][NP];
   const uint32_t N = a.states;
   const ScanLane<NS, LP> me(a.channels, a.groups, p.per_group, blockIdx.x % p.ctiles);
+  const uint32_t part = threadIdx.x % LP;
   const int64_t chunk = blockIdx.x / p.ctiles;
   const int64_t t0 = chunk * (int64_t)p.len, t1 = min(t0 + (int64_t)p.len, (int64_t)a.seq.tokens);
   const int64_t seq = a.seq.of(t0);
@@ -52,282 +55,354 @@ __global__ void __launch_bounds__(kScanThreads) sscan_chunk_back_kernel(SscanArg
   if (threadIdx.x == 0 && blockIdx.x % p.ctiles == 0) w.cut[chunk] = !spans ? 2 : end <= t1 ? 1 : 0;
   if (!spans) return;
   const int64_t hi = min(end, t1);
-  float r[NS], a2[NS];
-  load_states<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2);
-#pragma unroll
-  for (int j = 0; j < NS; ++j) a2[j] *= kLog2e;
-  zero_states(r);
+  f32x2 r[NS / 2], a2[NS / 2];
+  load_pairs<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2, kLog2e);
+  zero_pairs(r);
   if (end <= t1 && a.dfinal) {
     const int64_t slot = a.seq.slot(seq);
-    if (slot >= 0) load_states<NS, FULL>(a.dfinal + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, r);
+    if (slot >= 0) load_pairs<NS, FULL>(a.dfinal + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, r);
   }
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
   const T* dt = reinterpret_cast<const T*>(a.dt) + me.c;
   const T* dy = reinterpret_cast<const T*>(a.dy) + me.c;
-  const T* z = a.z ? reinterpret_cast<const T*>(a.z) + me.c : nullptr;
-  const T* cp = reinterpret_cast<const T*>(a.c) + (uint64_t)me.group * a.c_group;
+  const T* z = GATE ? reinterpret_cast<const T*>(a.z) + me.c : nullptr;
   float sum = 0.f;
-  for (int64_t te = hi; te > t0; te -= kScanTile) {  // tokens te - 1 down to te - kScanTile
-    __syncthreads();
-    for (int i = threadIdx.x; i < kScanTile * NP; i += kScanThreads) {
-      const uint32_t n = i % NP, k = i / NP;
-      const int64_t t = te - 1 - (int64_t)k;
-      sc[k][n] = t >= t0 && n < N ? to_f32(cp[(uint64_t)t * a.c_stride + n]) : 0.f;
-    }
-    __syncthreads();
-    for (int k = 0; k < kScanTile; k += U) {
-      T dr[U], gr[U], zr[U];
+  T dr[kOwn], gr[kOwn], zr[kOwn];
+  const auto load = [&](int64_t te) {  // own tokens of the batch that ends in front of te
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t t = te - 1 - (k + u);
-        if (t >= t0) {
-          dr[u] = dt[(uint64_t)t * a.dt_stride];
-          gr[u] = dy[(uint64_t)t * a.dy_stride];
-          if (z) zr[u] = z[(uint64_t)t * a.z_stride];
+    for (int j = 0; j < kOwn; ++j) {
+      const int64_t t = te - 1 - (j * LP + (int64_t)part);
+      if (t < t0) continue;
+      dr[j] = dt[(uint64_t)t * a.dt_stride];
+      gr[j] = dy[(uint64_t)t * a.dy_stride];
+      if (GATE) zr[j] = z[(uint64_t)t * a.z_stride];
+    }
+  };
+  StageBC<T, NP, 1, true> stage;
+  const auto above = [&](int64_t tb) { return tb >= t0 ? ~0u : ~first_bits(t0 - tb); };
+  stage.fetch(a, me.group, hi - kScanTile, above(hi - kScanTile));
+  stage.put(&sc[0][0][0]);
+  load(hi);
+  __syncthreads();
+  int buf = 0;
+  for (int64_t te = hi; te > t0; te -= kScanTile, buf ^= 1) {
+    stage.fetch(a, me.group, te - 2 * kScanTile, above(te - 2 * kScanTile));
+#pragma unroll 1
+    for (int k0 = 0; k0 < kScanTile; k0 += U) {
+      const int64_t left = te - k0 - t0;
+      if (left <= 0) break;
+      float s[kOwn], g[kOwn];
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) {
+        const bool live = j * LP + (int64_t)part < left;
+        s[j] = g[j] = 0.f;  // a token in front of the chunk changes nothing: e = 1
+        if (live) {
+          s[j] = to_f32(dr[j]) + bias;
+          if (a.softplus) s[j] = softplus(s[j]);
+          sum += s[j];
+          g[j] = to_f32(gr[j]);
+          if (GATE) {
+            const float zv = to_f32(zr[j]);
+            g[j] *= zv * sigmoid(zv);
+          }
         }
       }
+      load(te - k0 - U);
+      f32x2 e[NS / 2], en[NS / 2];
+      decay<NS>(from_lane<LP>(s[0], 0), a2, e);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (te - 1 - (k + u) < t0) break;
-        float s = to_f32(dr[u]) + bias;
-        if (a.softplus) s = softplus(s);
-        sum += s;
-        float g = to_f32(gr[u]);
-        if (z) {
-          const float zv = to_f32(zr[u]);
-          g *= zv * sigmoid(zv);
+      for (int k = 0; k < U; ++k) {
+        if (k + 1 < U) decay<NS>(from_lane<LP>(s[(k + 1) / LP], (k + 1) % LP), a2, en);
+        const float gv = from_lane<LP>(g[k / LP], k % LP);
+        const f32x2 gg = pair(gv, gv);
+        const float* row = &sc[buf][kScanTile - 1 - (k0 + k)][me.n0];
+#pragma unroll
+        for (int i = 0; i < NS / 2; i += 2) {
+          const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(row + 2 * i);
+          r[i] = mul2(e[i], fma2(cc.x, gg, r[i]));
+          r[i + 1] = mul2(e[i + 1], fma2(cc.y, gg, r[i + 1]));
         }
 #pragma unroll
-        for (int j = 0; j < NS; ++j) r[j] = ex2(s * a2[j]) * __fmaf_rn(sc[k + u][me.n0 + j], g, r[j]);
+        for (int i = 0; i < NS / 2; ++i) e[i] = en[i];
       }
     }
+    stage.put(&sc[buf ^ 1][0][0]);
+    __syncthreads();
   }
+  sum = sum_lanes<LP>(sum);
   if (!me.valid) return;
-  store_states<NS, FULL>(w.state + ((uint64_t)chunk * a.channels + me.c) * N, me.n0, N, r);
+  store_pairs<NS, FULL>(w.state + ((uint64_t)chunk * a.channels + me.c) * N, me.n0, N, r);
   if (me.first) w.sum[(uint64_t)chunk * a.channels + me.c] = sum;
 }
 
-// v[i] summed over the lanes that hold the same states of other channels; the
-// lane keeps the sums of `kept` of its states from index `at` on.
-template <int NS, int LP>
-struct LaneSum {
-  static constexpr int rounds() {
-    int r = 0;
-    for (int o = 16, cnt = NS; o >= LP && cnt > 1; o >>= 1, cnt /= 2) ++r;
-    return r;
+// Sums over a warp's channels.  For each of four tokens a warp's lanes leave
+// 8 states each in 1 KB of shared memory: row by row of channels, a row's
+// quads of states at slot ^ turn(row), which keeps both the lanes' stores (a
+// row after another) and the sums' loads (a slot's quads of several rows) on
+// different banks.  Adding in shared memory takes a fifth of the instructions
+// of exchanges between lanes.
+template <int LP>
+struct WarpSum {
+  static constexpr int kRows = 32 / LP, kSlots = 2 * LP, kShare = LP <= 4 ? 4 / LP : 1;  // lanes per sum
+  static constexpr int kItems = 4 * kSlots * kShare;
+  static __device__ __forceinline__ uint32_t turn(uint32_t row) {
+    return LP <= 4 ? (row >> (LP == 1 ? 2 : LP == 2 ? 1 : 0) & 1) * LP : 0;
   }
-  static constexpr int kept = NS >> rounds();
-  uint32_t at;
-  bool writes;
-  __device__ __forceinline__ LaneSum() {
-    const uint32_t lane = threadIdx.x & 31;
-    at = 0;
-    writes = true;
-    int cnt = NS;
-#pragma unroll
-    for (int o = 16; o >= LP; o >>= 1) {
-      if (cnt > 1) {
-        cnt /= 2;
-        if (lane & o) at += cnt;
-      } else if (lane & o) {
-        writes = false;
-      }
-    }
+  // Lane's states 0..7 of token k (0..3).
+  static __device__ __forceinline__ void put(float* v, int k, const f32x2 (&s)[4]) {
+    const uint32_t lane = threadIdx.x & 31, row = lane / LP, part = lane % LP;
+    ulonglong2* q = reinterpret_cast<ulonglong2*>(v) + k * 64 + row * kSlots;
+    q[part ^ turn(row)] = make_ulonglong2(s[0], s[1]);
+    q[(LP + part) ^ turn(row)] = make_ulonglong2(s[2], s[3]);
   }
-  __device__ __forceinline__ void operator()(float (&v)[NS]) const {
+  // The four tokens' sums to out[token * stride + state].
+  static __device__ __forceinline__ void add(const float* v, float* out, int stride) {
     const uint32_t lane = threadIdx.x & 31;
-    int cnt = NS;
+    __syncwarp();
 #pragma unroll
-    for (int o = 16; o >= LP; o >>= 1) {
-      if (cnt > 1) {
-        cnt /= 2;
-        const bool up = lane & o;
+    for (int it = 0; it < kItems / 32; ++it) {
+      const uint32_t item = it * 32 + lane, k = item / (kSlots * kShare), slot = item / kShare % kSlots, share = item % kShare;
+      const ulonglong2* q = reinterpret_cast<const ulonglong2*>(v) + k * 64;
+      f32x2 lo = 0ull, hi = 0ull;
 #pragma unroll
-        for (int j = 0; j < NS / 2; ++j) {
-          if (j < cnt) {
-            const float send = up ? v[j] : v[j + cnt], keep = up ? v[j + cnt] : v[j];
-            v[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-          }
-        }
-      } else {
-        v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      for (int i = 0; i < kRows / kShare; ++i) {
+        const uint32_t row = i * kShare + share;
+        const ulonglong2 t = q[row * kSlots + (slot ^ turn(row))];
+        lo = add2(lo, t.x);
+        hi = add2(hi, t.y);
       }
+      float s[4];
+      unpair(lo, s[0], s[1]);
+      unpair(hi, s[2], s[3]);
+#pragma unroll
+      for (int o = 1; o < kShare; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+      if (share == 0)
+        *reinterpret_cast<float4*>(out + k * stride + slot % LP * 8 + slot / LP * 4) = make_float4(s[0], s[1], s[2], s[3]);
     }
+    __syncwarp();
   }
 };
 
-template <class T, int NS, int LP, bool FULL>
-__global__ void __launch_bounds__(kScanThreads) sscan_back_kernel(SscanArgs a, ScanPlan p, BackWork w) {
-  constexpr int NP = NS * LP, K = (int)kMarkEvery;
-  using Sum = LaneSum<NS, LP>;
-  __shared__ __align__(16) float bc[kScanTile][2][NP];
-  __shared__ float red[2][kWarps][K][2][NP];
+template <int NP>
+struct BackShared {
+  float bc[2][kScanTile][2][NP];
+  float red[2][kWarps][2][kBlock][NP];  // dB's sums, then dC's
+  float sum[kWarps][4][256];
+};
+
+// A block of kBlock tokens at a time, last ones first: forwards from its mark
+// with decays and states kept in registers, then backwards.
+template <class T, int LP, bool FULL, bool GATE>
+__global__ void __launch_bounds__(kScanThreads, kResident) sscan_back_kernel(SscanArgs a, ScanPlan p, BackWork w) {
+  constexpr int NS = 8, NP = NS * LP, K = kBlock, kOwn = K / LP;
+  extern __shared__ __align__(16) unsigned char shared_bytes[];
+  BackShared<NP>& sh = *reinterpret_cast<BackShared<NP>*>(shared_bytes);
   const uint32_t N = a.states;
   const ScanLane<NS, LP> me(a.channels, a.groups, p.per_group, blockIdx.x % p.ctiles);
+  const uint32_t part = threadIdx.x % LP, warp = threadIdx.x >> 5;
   const int64_t chunk = blockIdx.x / p.ctiles;
   const int64_t t0 = chunk * (int64_t)p.len, t1 = min(t0 + (int64_t)p.len, (int64_t)a.seq.tokens);
-  const uint32_t warp = threadIdx.x >> 5;
-  const Sum lane_sum;
-  float a2[NS], r[NS], da[NS];
-  load_states<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2);
-#pragma unroll
-  for (int j = 0; j < NS; ++j) a2[j] *= kLog2e;
-  zero_states(r);
-  zero_states(da);
+  float* sums = &sh.sum[warp][0][0];
+  f32x2 a2[4], r[4], da[4];
+  load_pairs<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2, kLog2e);
+  zero_pairs(r);
+  zero_pairs(da);
   const uint64_t row = ((uint64_t)chunk * a.channels + me.c) * N;
-  if (p.carry && me.valid) load_states<NS, FULL>(w.scan.state + row, me.n0, N, r);
+  if (p.carry && me.valid) load_pairs<NS, FULL>(w.scan.state + row, me.n0, N, r);
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
   const float dskip = a.d ? a.d[me.c] : 0.f;
   float dd = 0.f, dbias = 0.f;
-  const T* x = reinterpret_cast<const T*>(a.x) + me.c;
-  const T* dt = reinterpret_cast<const T*>(a.dt) + me.c;
-  const T* dy = reinterpret_cast<const T*>(a.dy) + me.c;
-  const T* z = a.z ? reinterpret_cast<const T*>(a.z) + me.c : nullptr;
-  T* dx = reinterpret_cast<T*>(a.dx) + me.c;
-  T* ddt = reinterpret_cast<T*>(a.ddt) + me.c;
-  T* dz = a.z ? reinterpret_cast<T*>(a.dz) + me.c : nullptr;
-  int buf = 0;
+  T xr[kOwn], dr[kOwn], gr[kOwn], zr[kOwn];
+  // Own tokens of the block from t on that `live` names.
+  const auto load = [&](int64_t t, uint32_t live) {
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      if (!(live >> (j * LP + part) & 1)) continue;
+      const uint64_t at = (uint64_t)t + j * LP + part;
+      xr[j] = reinterpret_cast<const T*>(a.x)[at * a.x_stride + me.c];
+      dr[j] = reinterpret_cast<const T*>(a.dt)[at * a.dt_stride + me.c];
+      gr[j] = reinterpret_cast<const T*>(a.dy)[at * a.dy_stride + me.c];
+      if (GATE) zr[j] = reinterpret_cast<const T*>(a.z)[at * a.z_stride + me.c];
+    }
+  };
+  const auto mark_of = [&](int64_t t) {
+    return a.marks + ((uint64_t)(t / K) * a.channels + me.c) * N;
+  };
+  const auto state_row = [&](int64_t seq) {
+    const int64_t slot = a.seq.slot(seq);
+    return slot < 0 || !me.valid ? -1 : (int64_t)(((uint64_t)slot * a.channels + me.c) * N);
+  };
 
   const int64_t tiles = (t1 - t0 + kScanTile - 1) / kScanTile;
-  for (int64_t tile = tiles - 1; tile >= 0; --tile) {
+  StageBC<T, NP, 2> stage;
+  TileMarks m, before;
+  if (tiles > 0) {
+    m = tile_marks(a.seq, t0 + (tiles - 1) * kScanTile, t1);
+    stage.fetch(a, me.group, t0 + (tiles - 1) * kScanTile, m.live);
+    stage.put(&sh.bc[0][0][0][0]);
+    load(t0 + tiles * kScanTile - K, m.live >> (kScanTile - K));
+  }
+  __syncthreads();
+  int buf = 0, out = 0;
+  for (int64_t tile = tiles - 1; tile >= 0; --tile, buf ^= 1, m = before) {
     const int64_t tb = t0 + tile * kScanTile;
-    const TileMarks m = tile_marks(a.seq, tb, t1);
-    if (m.live == 0) continue;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kScanTile * 2 * NP; i += kScanThreads) {
-      const uint32_t n = i % NP, which = i / NP & 1, k = i / (NP * 2);
-      const int64_t t = tb + k;
-      float v = 0.f;
-      if ((m.live >> k & 1) && n < N) {
-        const T* q = reinterpret_cast<const T*>(which ? a.c : a.b);
-        v = to_f32(q[(uint64_t)t * (which ? a.c_stride : a.b_stride) + (uint64_t)me.group * (which ? a.c_group : a.b_group) + n]);
-      }
-      bc[k][which][n] = v;
+    before.live = 0;
+    if (tile > 0) {
+      before = tile_marks(a.seq, tb - kScanTile, t1);
+      stage.fetch(a, me.group, tb - kScanTile, before.live);
     }
-    __syncthreads();
+#pragma unroll 1
     for (int k0 = kScanTile - K; k0 >= 0; k0 -= K) {
-      const uint32_t live = m.live >> k0 & ((1u << K) - 1);
-      if (!live) continue;
-      float xv[K], sv[K], up[K], gv[K], slope[K];
-      float hp[K][NS], e[K][NS], h[NS];
-      // Forwards from the mark.
-      zero_states(h);
-      if ((live & 1) && me.valid)
-        load_states<NS, FULL>(a.marks + ((uint64_t)((tb + k0) / K) * a.channels + me.c) * N, me.n0, N, h);
-      float zv[K];
+      const uint32_t live = m.live >> k0 & ((1u << K) - 1), start = m.start >> k0, end = m.end >> k0;
+      const uint32_t live_next = k0 ? m.live >> (k0 - K) : before.live >> (kScanTile - K);
+      // This lane's own tokens: steps, gates; those that are no tokens change nothing (e = 1).
+      float s[kOwn], sx[kOwn], g[kOwn], xv[kOwn], slope[kOwn], gg[kOwn];
 #pragma unroll
-      for (int u = 0; u < K; ++u) {
-        xv[u] = sv[u] = up[u] = zv[u] = 0.f;
-        if ((live >> u & 1) && me.valid) {
-          const uint64_t t = (uint64_t)(tb + k0 + u);
-          xv[u] = to_f32(x[t * a.x_stride]);
-          sv[u] = to_f32(dt[t * a.dt_stride]) + bias;
-          up[u] = to_f32(dy[t * a.dy_stride]);
-          if (z) zv[u] = to_f32(z[t * a.z_stride]);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < K; ++u) {
-        const int k = k0 + u;
-        slope[u] = 1.f;
-        if (a.softplus) {
-          slope[u] = sigmoid(sv[u]);
-          sv[u] = softplus(sv[u]);
-        }
-        if ((m.start >> k & 1) && u) {
-          zero_states(h);
-          const int64_t slot = a.state ? a.seq.slot(tile_seq(m, k)) : -1;
-          if (slot >= 0 && me.valid)
-            load_states<NS, FULL>(a.state + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, h);
-        }
-        const float sx = sv[u] * xv[u];
-        float o = 0.f;
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-          hp[u][j] = h[j];
-          e[u][j] = ex2(sv[u] * a2[j]);
-          float add = sx * bc[k][0][me.n0 + j];
-          if (!FULL && me.n0 + j >= N) add = 0.f;
-          h[j] = __fmaf_rn(e[u][j], h[j], add);
-          o = __fmaf_rn(bc[k][1][me.n0 + j], h[j], o);
-        }
-        if (z) {
-          o = sum_lanes<LP>(o);
-          if (a.d) o = __fmaf_rn(dskip, xv[u], o);
-          const float sig = sigmoid(zv[u]);
-          if ((live >> u & 1) && me.valid && me.first)
-            dz[(uint64_t)(tb + k) * a.dz_stride] = from_f32<T>(up[u] * o * gate_grad(zv[u], sig));
-          up[u] *= zv[u] * sig;
-        }
-        gv[u] = up[u];
-        float v[NS];
-#pragma unroll
-        for (int j = 0; j < NS; ++j) v[j] = gv[u] * h[j];
-        lane_sum(v);
-        if (lane_sum.writes)
-#pragma unroll
-          for (int j = 0; j < Sum::kept; ++j) red[buf][warp][u][1][me.n0 + lane_sum.at + j] = v[j];
-      }
-      // Backwards.
-#pragma unroll
-      for (int u = K - 1; u >= 0; --u) {
-        const int k = k0 + u;
-        if (m.end >> k & 1) {
-          zero_states(r);
-          const int64_t slot = a.dfinal ? a.seq.slot(tile_seq(m, k)) : -1;
-          if (slot >= 0 && me.valid)
-            load_states<NS, FULL>(a.dfinal + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, r);
-        }
-        const float sx = sv[u] * xv[u];
-        float gb = 0.f, ga = 0.f, v[NS];
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-          const float g = __fmaf_rn(bc[k][1][me.n0 + j], gv[u], r[j]);
-          gb = __fmaf_rn(g, bc[k][0][me.n0 + j], gb);
-          r[j] = e[u][j] * g;
-          const float through = r[j] * hp[u][j];
-          ga = __fmaf_rn(through, a2[j], ga);
-          da[j] = __fmaf_rn(through, sv[u], da[j]);
-          v[j] = g * sx;
-        }
-        lane_sum(v);
-        if (lane_sum.writes)
-#pragma unroll
-          for (int j = 0; j < Sum::kept; ++j) red[buf][warp][u][0][me.n0 + lane_sum.at + j] = v[j];
-        gb = sum_lanes<LP>(gb);
-        ga = sum_lanes<LP>(ga);
-        if (live >> u & 1) {
-          const float ds = __fmaf_rn(ga, 1.0f / kLog2e, xv[u] * gb) * slope[u];
-          dd = __fmaf_rn(gv[u], xv[u], dd);
-          dbias += ds;
-          if (me.valid && me.first) {
-            const uint64_t t = (uint64_t)(tb + k);
-            dx[t * a.dx_stride] = from_f32<T>(__fmaf_rn(dskip, gv[u], sv[u] * gb));
-            ddt[t * a.ddt_stride] = from_f32<T>(ds);
+      for (int j = 0; j < kOwn; ++j) {
+        s[j] = sx[j] = g[j] = xv[j] = slope[j] = gg[j] = 0.f;
+        if ((live >> (j * LP + part) & 1) && me.valid) {
+          xv[j] = to_f32(xr[j]);
+          s[j] = to_f32(dr[j]) + bias;
+          slope[j] = 1.f;
+          if (a.softplus) {
+            slope[j] = sigmoid(s[j]);
+            s[j] = softplus(s[j]);
+          }
+          sx[j] = s[j] * xv[j];
+          g[j] = to_f32(gr[j]);
+          if (GATE) {
+            const float zv = to_f32(zr[j]), sig = sigmoid(zv);
+            gg[j] = g[j] * gate_grad(zv, sig);
+            g[j] *= zv * sig;
           }
         }
-        if ((m.start >> k & 1) && a.dstate) {
-          const int64_t slot = a.seq.slot(tile_seq(m, k));
-          if (slot >= 0 && me.valid)
-            store_states<NS, FULL>(a.dstate + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, r);
+      }
+      f32x2 h[4], hp[K][4], e[K][4];
+      zero_pairs(h);
+      if ((live & 1) && me.valid) load_pairs<NS, FULL>(mark_of(tb + k0), me.n0, N, h);
+      load(tb + k0 - K, live_next);
+      if (live) {
+        // Forwards.
+        float o[LP];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int j = k / LP, q = k % LP;
+          if (k && (start >> k & 1)) {
+            zero_pairs(h);
+            const int64_t at = a.state ? state_row(tile_seq(m, k0 + k)) : -1;
+            if (at >= 0) load_pairs<NS, FULL>(a.state + at, me.n0, N, h);
+          }
+          decay<NS>(from_lane<LP>(s[j], q), a2, e[k]);
+          const float xq = from_lane<LP>(sx[j], q), gq = from_lane<LP>(g[j], q);
+          const f32x2 xx = pair(xq, xq), gv = pair(gq, gq);
+          f32x2 v[4], oo = 0ull;
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sh.bc[buf][k0 + k][0][me.n0 + 2 * i]);
+            f32x2 add[2] = {mul2(xx, bb.x), mul2(xx, bb.y)};
+            if (!FULL) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                float lo, hi;
+                unpair(add[u], lo, hi);
+                const uint32_t n = me.n0 + 2 * (i + u);
+                add[u] = pair(n < N ? lo : 0.f, n + 1 < N ? hi : 0.f);
+              }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              hp[k][i + u] = h[i + u];
+              h[i + u] = fma2(e[k][i + u], h[i + u], add[u]);
+              v[i + u] = mul2(gv, h[i + u]);
+            }
+            if (GATE) {
+              const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sh.bc[buf][k0 + k][1][me.n0 + 2 * i]);
+              oo = fma2(cc.x, h[i], oo);
+              oo = fma2(cc.y, h[i + 1], oo);
+            }
+          }
+          WarpSum<LP>::put(sums, k & 3, v);
+          if ((k & 3) == 3) WarpSum<LP>::add(sums, &sh.red[out][warp][1][k - 3][0], NP);
+          if (GATE) {
+            o[q] = sum2(oo);
+            if (q == LP - 1) {
+              const float pre = __fmaf_rn(dskip, xv[j], scatter_sum<LP>(o, part));
+              if ((live >> (j * LP + part) & 1) && me.valid)
+                reinterpret_cast<T*>(a.dz)[(uint64_t)(tb + k0 + j * LP + part) * a.dz_stride + me.c] = from_f32<T>(gg[j] * pre);
+            }
+          }
         }
-        if (m.start >> k & 1) zero_states(r);  // rows in front of it belong to no sequence, or end one
+        // Backwards.
+        float gb[LP], ga[LP];
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k) {
+          const int j = k / LP, q = k % LP;
+          if (end >> k & 1) {
+            zero_pairs(r);
+            const int64_t at = a.dfinal ? state_row(tile_seq(m, k0 + k)) : -1;
+            if (at >= 0) load_pairs<NS, FULL>(a.dfinal + at, me.n0, N, r);
+          }
+          const float sq = from_lane<LP>(s[j], q), xq = from_lane<LP>(sx[j], q), gq = from_lane<LP>(g[j], q);
+          const f32x2 ss = pair(sq, sq), xx = pair(xq, xq), gv = pair(gq, gq);
+          f32x2 v[4], gb2 = 0ull, ga2 = 0ull;
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sh.bc[buf][k0 + k][0][me.n0 + 2 * i]);
+            const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sh.bc[buf][k0 + k][1][me.n0 + 2 * i]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const f32x2 gh = fma2(u ? cc.y : cc.x, gv, r[i + u]);
+              gb2 = fma2(gh, u ? bb.y : bb.x, gb2);
+              r[i + u] = mul2(e[k][i + u], gh);
+              const f32x2 through = mul2(r[i + u], hp[k][i + u]);
+              ga2 = fma2(through, a2[i + u], ga2);
+              da[i + u] = fma2(through, ss, da[i + u]);
+              v[i + u] = mul2(gh, xx);
+            }
+          }
+          WarpSum<LP>::put(sums, k & 3, v);
+          if ((k & 3) == 0) WarpSum<LP>::add(sums, &sh.red[out][warp][0][k][0], NP);
+          gb[q] = sum2(gb2);
+          ga[q] = sum2(ga2);
+          if (q == 0) {
+            const float gbs = scatter_sum<LP>(gb, part), gas = scatter_sum<LP>(ga, part);
+            if ((live >> (j * LP + part) & 1) && me.valid) {
+              const float ds = __fmaf_rn(gas, 1.0f / kLog2e, xv[j] * gbs) * slope[j];
+              dd = __fmaf_rn(g[j], xv[j], dd);
+              dbias += ds;
+              const uint64_t t = (uint64_t)(tb + k0 + j * LP + part);
+              reinterpret_cast<T*>(a.dx)[t * a.dx_stride + me.c] = from_f32<T>(__fmaf_rn(dskip, g[j], s[j] * gbs));
+              reinterpret_cast<T*>(a.ddt)[t * a.ddt_stride + me.c] = from_f32<T>(ds);
+            }
+          }
+          if (start >> k & 1) {
+            const int64_t at = a.dstate ? state_row(tile_seq(m, k0 + k)) : -1;
+            if (at >= 0) store_pairs<NS, FULL>(a.dstate + at, me.n0, N, r);
+            zero_pairs(r);  // rows in front of it belong to no sequence, or end one
+          }
+        }
       }
       __syncthreads();
       for (int i = threadIdx.x; i < K * 2 * NP; i += kScanThreads) {
-        const uint32_t n = i % NP, which = i / NP & 1, u = i / (2 * NP);
-        if (n >= N || !(live >> u & 1)) continue;
-        float s = 0.f;
+        const uint32_t n = i % NP, k = i / NP % K, which = i / (NP * K);
+        if (n >= N || !(live >> k & 1)) continue;
+        float v = 0.f;
 #pragma unroll
-        for (int q = 0; q < kWarps; ++q) s += red[buf][q][u][which][n];
-        const uint64_t t = (uint64_t)(tb + k0 + u);
-        w.bc[((((uint64_t)me.channel_tile * a.seq.tokens + t) * a.groups + me.group) * 2 + which) * N + n] = s;
+        for (int q = 0; q < kWarps; ++q) v += sh.red[out][q][which][k][n];
+        const uint64_t t = (uint64_t)(tb + k0 + k);
+        w.bc[((((uint64_t)me.channel_tile * a.seq.tokens + t) * a.groups + me.group) * 2 + which) * N + n] = v;
       }
-      buf ^= 1;  // the next block of tokens writes the other one while this is read
+      out ^= 1;  // the next block of tokens writes the other one while this is read
     }
+    if (tile > 0) stage.put(&sh.bc[buf ^ 1][0][0][0]);
+    __syncthreads();
   }
+  dd = sum_lanes<LP>(dd);
+  dbias = sum_lanes<LP>(dbias);
   if (!me.valid) return;
-  store_states<NS, FULL>(w.da + row, me.n0, N, da);
+  store_pairs<NS, FULL>(w.da + row, me.n0, N, da);
   if (me.first) {
     w.dd[(uint64_t)chunk * 2 * a.channels + me.c] = dd;
     w.dd[((uint64_t)chunk * 2 + 1) * a.channels + me.c] = dbias;
@@ -339,12 +414,11 @@ __global__ void __launch_bounds__(kScanThreads) sscan_back_kernel(SscanArgs a, S
     const int64_t begin = a.seq.begin(i);
     if (begin >= t1 && !last) break;
     if (a.seq.begin(i + 1) > begin) continue;
-    const int64_t slot = a.seq.slot(i);
-    if (slot < 0) continue;
-    zero_states(r);
-    const uint64_t at = ((uint64_t)slot * a.channels + me.c) * N;
-    if (a.dfinal) load_states<NS, FULL>(a.dfinal + at, me.n0, N, r);
-    store_states<NS, FULL>(a.dstate + at, me.n0, N, r);
+    const int64_t at = state_row(i);
+    if (at < 0) continue;
+    zero_pairs(r);
+    if (a.dfinal) load_pairs<NS, FULL>(a.dfinal + at, me.n0, N, r);
+    store_pairs<NS, FULL>(a.dstate + at, me.n0, N, r);
   }
 }
 
@@ -370,7 +444,7 @@ bool aligned16(const void* p) { return reinterpret_cast<uint64_t>(p) % 16 == 0; 
 constexpr uint32_t lanes_of(uint32_t states) { return states <= 8 ? 1 : states <= 16 ? 2 : states <= 32 ? 4 : 8; }
 
 ScanPlan plan_of(uint64_t tokens, uint32_t channels, uint32_t states, uint64_t n_seq, uint32_t groups, bool ragged) {
-  return scan_plan(tokens, channels, groups, n_seq, ragged, {lanes_of(states), lanes_of(states)});
+  return scan_plan(tokens, channels, groups, n_seq, ragged, {lanes_of(states), lanes_of(states), kResident});
 }
 
 uint64_t back_work(const ScanPlan& p, uint64_t tokens, uint32_t channels, uint32_t states, uint32_t groups, void* base,
@@ -385,21 +459,36 @@ uint64_t back_work(const ScanPlan& p, uint64_t tokens, uint32_t channels, uint32
   return at + scan_round((uint64_t)p.per_group * tokens * groups * 2 * states * 4);
 }
 
-template <class T, int NS, int LP, bool FULL>
+template <class T, int LP, bool FULL, bool GATE>
 cudaError_t go(const SscanArgs& a, cudaStream_t s) {
   const ScanPlan p = plan_of(a.seq.tokens, a.channels, a.states, a.seq.n_seq, a.groups, a.seq.seq_ptr != nullptr);
   BackWork w{};
   back_work(p, a.seq.tokens, a.channels, a.states, a.groups, a.work, &w);
   const uint64_t grid = p.chunks * p.ctiles;
   if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
+  cudaError_t e;
   if (p.carry) {
-    sscan_chunk_back_kernel<T, NS, LP, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w.scan);
-    launch_sscan_fold_back(a.a, w.scan, p.chunks, a.channels, a.states, s);
+    // The same chunks with up to 16 states a lane: there is no history to keep.
+    constexpr int CL = LP <= 2 ? 1 : LP / 2, CS = LP * 8 / CL;
+    ScanPlan q = p;
+    const uint32_t cpg = a.channels / a.groups;
+    q.lanes = CL;
+    q.per_group = (cpg + kScanThreads / CL - 1) / (kScanThreads / CL);
+    q.ctiles = q.per_group * a.groups;
+    sscan_chunk_back_kernel<T, CS, CL, FULL, GATE><<<(unsigned)(p.chunks * q.ctiles), kScanThreads, 0, s>>>(a, q, w.scan);
+    e = launch_sscan_fold_back(a.a, w.scan, p.chunks, a.channels, a.states, s);
+    if (e != cudaSuccess) return e;
   }
-  sscan_back_kernel<T, NS, LP, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w);
+  constexpr int bytes = sizeof(BackShared<8 * LP>);
+  const auto kernel = sscan_back_kernel<T, LP, FULL, GATE>;
+  if (bytes > 48 * 1024) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<(unsigned)grid, kScanThreads, bytes, s>>>(a, p, w);
   const uint64_t cells = a.seq.tokens * a.groups * 2 * a.states;
   if (cells) sscan_bc_kernel<T><<<(unsigned)((cells + 255) / 256), 256, 0, s>>>(a, w.bc, p.per_group);
-  cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const uint64_t as = (uint64_t)a.channels * a.states;
   e = launch_reduce_rows(w.da, p.chunks, as, as, a.da, nullptr, s);
@@ -408,19 +497,22 @@ cudaError_t go(const SscanArgs& a, cudaStream_t s) {
   return e;
 }
 
+template <class T, int LP>
+cudaError_t by_form(const SscanArgs& a, cudaStream_t s) {
+  const bool full = a.states == 8 * LP && aligned16(a.a) && aligned16(a.state) && aligned16(a.dstate) && aligned16(a.dfinal) &&
+                    aligned16(a.marks) && aligned16(a.work);
+  if (full) return a.z ? go<T, LP, true, true>(a, s) : go<T, LP, true, false>(a, s);
+  return a.z ? go<T, LP, false, true>(a, s) : go<T, LP, false, false>(a, s);
+}
+
 template <class T>
 cudaError_t by_states(const SscanArgs& a, cudaStream_t s) {
-  const uint32_t N = a.states;
-  const bool al = aligned16(a.a) && aligned16(a.state) && aligned16(a.dstate) && aligned16(a.dfinal) && aligned16(a.marks) &&
-                  aligned16(a.work);
-  if (N == 8 && al) return go<T, 8, 1, true>(a, s);
-  if (N == 16 && al) return go<T, 8, 2, true>(a, s);
-  if (N == 32 && al) return go<T, 8, 4, true>(a, s);
-  if (N == 64 && al) return go<T, 8, 8, true>(a, s);
-  if (N <= 8) return go<T, 8, 1, false>(a, s);
-  if (N <= 16) return go<T, 8, 2, false>(a, s);
-  if (N <= 32) return go<T, 8, 4, false>(a, s);
-  return go<T, 8, 8, false>(a, s);
+  switch (lanes_of(a.states)) {
+    case 1: return by_form<T, 1>(a, s);
+    case 2: return by_form<T, 2>(a, s);
+    case 4: return by_form<T, 4>(a, s);
+    default: return by_form<T, 8>(a, s);
+  }
 }
 
 }  // namespace
