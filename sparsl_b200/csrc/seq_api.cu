@@ -92,7 +92,7 @@ struct Call {
       fail(SPARSL_ERR_LENGTH, "row stride", std::string(name) + ": rows overlap (the stride is below the row's length)");
       return;
     }
-    if (stride > kMostRows * 4) {
+    if (stride > kMostStride) {
       fail(SPARSL_ERR_LENGTH, "row stride", std::string(name) + ": the row stride is too large");
       return;
     }
@@ -288,7 +288,7 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
     const uint64_t row = ch * n;
     const auto bc = [&](const char* name, const sparsl_rows& r, uint64_t group, bool out) {
       k.want(g == 1 || group >= n, SPARSL_ERR_LENGTH, "group stride", "the runs of b or c overlap");
-      k.want(group <= kMostRows, SPARSL_ERR_LENGTH, "group stride", "the group stride is too large");
+      k.want(group <= kMostStride, SPARSL_ERR_LENGTH, "group stride", "the group stride is too large");
       k.rows(name, r, t, (g == 1 ? 0 : (g - 1) * group) + n, e, out);
     };
     k.rows("x", p->x, t, ch, e, false);
@@ -320,6 +320,10 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
     a.a = p->a;
     a.d = p->d;
     a.dt_bias = p->dt_bias;
+    const auto bytes = [&](const sparsl_rows& r) { return (uint32_t)(r.stride * e); };
+    a.x_row = bytes(p->x);
+    a.dt_row = bytes(p->dt);
+    a.z_row = bytes(p->z);
     a.state = step ? nullptr : p->state;
     a.work = p->workspace;
     a.marks = step ? nullptr : static_cast<float*>(p->checkpoints);
@@ -339,6 +343,10 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
       k.add("dfinal_state", p->dfinal_state, p->seqs.n_slots, row, row, 4, false, true);
       k.scratch("workspace", p->workspace, p->workspace_bytes, sscan_backward_bytes(t, ch, p->states, p->seqs.n_seq, p->groups));
       k.apart();
+      a.dy_row = bytes(p->dy);
+      a.dx_row = bytes(p->dx);
+      a.ddt_row = bytes(p->ddt);
+      a.dz_row = bytes(p->dz);
       a.dy = p->dy.p;
       a.dx = p->dx.p;
       a.ddt = p->ddt.p;
@@ -366,6 +374,7 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
     k.apart(step ? nullptr : p->state);
     a.y = p->y.p;
     a.y_stride = p->y.stride;
+    a.y_row = bytes(p->y);
     a.final_state = p->final_state;
     if (k.rc != SPARSL_OK || !p->seqs.n_seq) return k.rc;
     return k.done(step ? launch_sscan_step(a, stream_of(d, stream)) : launch_sscan(a, stream_of(d, stream)));

@@ -17,7 +17,6 @@
 namespace sparsl {
 namespace {
 
-constexpr int kAhead = 8;  // tokens in a batch: the next batch's rows are loaded while one is computed
 constexpr uint32_t kResident = 4;  // blocks an SM holds, at 128 registers a thread
 
 // One token: h <- e h + (s x) B.
@@ -41,37 +40,17 @@ __device__ __forceinline__ void advance(const f32x2 (&e)[NS / 2], float sx, cons
   }
 }
 
-// Rows of a batch, one token in LP of them per lane: the lanes that share a
-// channel divide a token's own work (step, gate, output) among them.
-template <class T, int LP>
-struct Batch {
-  static constexpr int kOwn = kAhead / LP;
-  T x[kOwn], dt[kOwn], z[kOwn];
-  template <bool GATE>
-  __device__ __forceinline__ void load(const T* px, const T* pdt, const T* pz, const SscanArgs& a) {
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-      x[j] = *px;
-      dt[j] = *pdt;
-      px += LP * a.x_stride;
-      pdt += LP * a.dt_stride;
-      if (GATE) {
-        z[j] = *pz;
-        pz += LP * a.z_stride;
-      }
-    }
-  }
-};
-
 // The state that a chunk hands to the next one: its last sequence's, from that
 // sequence's start in it or from zero.
 template <class T, int NS, int LP, bool FULL>
-__global__ void __launch_bounds__(kScanThreads, kResident) sscan_chunk_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
-  constexpr int NP = NS * LP;
+__global__ void __launch_bounds__(kScanThreads, kResident) sscan_chunk_kernel(SscanArgs a, ScanPlan p, ScanWork w, bool aligned) {
+  constexpr int NP = NS * LP, K = kBatch, kOwn = K / LP;
+  using Rows = WarpRows<T, LP>;
   __shared__ __align__(16) float bc[2][kScanTile][NP];
+  __shared__ __align__(16) T rows[kScanThreads / 32][2][2][K][Rows::kCols];
   const uint32_t N = a.states;
   const ScanLane<NS, LP> me(a.channels, a.groups, p.per_group, blockIdx.x % p.ctiles);
-  const uint32_t part = threadIdx.x % LP;
+  const uint32_t part = threadIdx.x % LP, col = threadIdx.x % 32 / LP;
   const int64_t chunk = blockIdx.x / p.ctiles;
   const int64_t t0 = chunk * (int64_t)p.len, t1 = min(t0 + (int64_t)p.len, (int64_t)a.seq.tokens);
   const int64_t seq = a.seq.of(t1 - 1);
@@ -90,58 +69,48 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_chunk_kernel(Ss
     if (w.start && me.valid) store_pairs<NS, FULL>(w.start + row, me.n0, N, h);
   }
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
-  const T* x = reinterpret_cast<const T*>(a.x) + me.c;
-  const T* dt = reinterpret_cast<const T*>(a.dt) + me.c;
   float sum = 0.f;
   StageBC<T, NP, 1> stage;
-  Batch<T, LP> now, next;
   const int64_t from = max(begin, t0);
+  const RowsIn arrays[2] = {{a.x, a.x_row}, {a.dt, a.dt_row}};
+  T(*const stages)[2][K][Rows::kCols] = rows[threadIdx.x / 32];
+  const auto fetch = [&](int at, int64_t t) {
+    Rows::in(stages[at], arrays, t, first_bits(t1 - t), me.warp_c, me.warp_cols, aligned);
+    copies_issued();
+  };
   stage.fetch(a, me.group, from, first_bits(t1 - from));
+  fetch(0, from);
   stage.put(&bc[0][0][0]);
-  const T* px = x + (uint64_t)(from + part) * a.x_stride;
-  const T* pdt = dt + (uint64_t)(from + part) * a.dt_stride;
-  if (t1 - from >= kAhead) next.template load<false>(px, pdt, nullptr, a);
   __syncthreads();
-  int buf = 0;
+  int buf = 0, at = 0;
   for (int64_t tb = from; tb < t1; tb += kScanTile, buf ^= 1) {
     stage.fetch(a, me.group, tb + kScanTile, first_bits(t1 - tb - kScanTile));
 #pragma unroll 1
-    for (int k0 = 0; k0 < kScanTile; k0 += kAhead) {
+    for (int k0 = 0; k0 < kScanTile; k0 += K, at ^= 1) {
       const int64_t left = t1 - tb - k0;  // the tokens not done
       if (left <= 0) break;
-      now = next;
-      px += kAhead * a.x_stride;
-      pdt += kAhead * a.dt_stride;
-      if (left >= 2 * kAhead) next.template load<false>(px, pdt, nullptr, a);
-      if (left >= kAhead) {
-        float s[Batch<T, LP>::kOwn], sx[Batch<T, LP>::kOwn];
+      copies_done();
+      fetch(at ^ 1, tb + k0 + K);
+      const T(&in)[2][K][Rows::kCols] = stages[at];
+      float s[kOwn], sx[kOwn];
 #pragma unroll
-        for (int j = 0; j < Batch<T, LP>::kOwn; ++j) {
-          s[j] = to_f32(now.dt[j]) + bias;
+      for (int j = 0; j < kOwn; ++j) {
+        s[j] = sx[j] = 0.f;  // a token behind the chunk changes nothing: its decay is 1
+        if (j * LP + (int64_t)part < left) {
+          s[j] = to_f32(in[1][j * LP + part][col]) + bias;
           if (a.softplus) s[j] = softplus(s[j]);
+          sx[j] = s[j] * to_f32(in[0][j * LP + part][col]);
           sum += s[j];
-          sx[j] = s[j] * to_f32(now.x[j]);
         }
-        f32x2 e[NS / 2], en[NS / 2];
-        decay<NS>(from_lane<LP>(s[0], 0), a2, e);
+      }
+      f32x2 e[NS / 2], en[NS / 2];
+      decay<NS>(from_lane<LP>(s[0], 0), a2, e);
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {  // a token's exponentials are under way while the one before it is added
-          if (k + 1 < kAhead) decay<NS>(from_lane<LP>(s[(k + 1) / LP], (k + 1) % LP), a2, en);
-          advance<NS, FULL>(e, from_lane<LP>(sx[k / LP], k % LP), &bc[buf][k0 + k][me.n0], me.n0, N, h);
+      for (int k = 0; k < K; ++k) {  // a token's exponentials are under way while the one before it is added
+        if (k + 1 < K) decay<NS>(from_lane<LP>(s[(k + 1) / LP], (k + 1) % LP), a2, en);
+        advance<NS, FULL>(e, from_lane<LP>(sx[k / LP], k % LP), &bc[buf][k0 + k][me.n0], me.n0, N, h);
 #pragma unroll
-          for (int i = 0; i < NS / 2; ++i) e[i] = en[i];
-        }
-      } else {
-#pragma unroll 1
-        for (int k = 0; k < (int)left; ++k) {
-          const uint64_t t = (uint64_t)(tb + k0 + k);
-          float s = to_f32(dt[t * a.dt_stride]) + bias;
-          if (a.softplus) s = softplus(s);
-          if (part == 0) sum += s;
-          f32x2 e[NS / 2];
-          decay<NS>(s, a2, e);
-          advance<NS, FULL>(e, s * to_f32(x[t * a.x_stride]), &bc[buf][k0 + k][me.n0], me.n0, N, h);
-        }
+        for (int i = 0; i < NS / 2; ++i) e[i] = en[i];
       }
     }
     stage.put(&bc[buf ^ 1][0][0]);
@@ -199,17 +168,19 @@ __device__ __forceinline__ float dot(const float* c, const f32x2 (&h)[NS / 2]) {
   return sum2(add2(o, p));
 }
 
-// The main pass over one chunk, in batches of kAhead tokens.  A batch inside one
-// sequence takes the straight path, its rows fetched while the batch before it
-// was computed; one in which a sequence begins or ends elsewhere than at its
-// edges goes token by token.
+// The main pass over one chunk, in batches of eight tokens.  A batch inside one
+// sequence takes the straight path; one in which a sequence begins or ends
+// elsewhere than at its edges goes token by token.
 template <class T, int NS, int LP, bool FULL, bool GATE>
-__global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
-  constexpr int NP = NS * LP;
+__global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArgs a, ScanPlan p, ScanWork w, bool aligned) {
+  constexpr int NP = NS * LP, K = kBatch, kOwn = K / LP, A = GATE ? 3 : 2;
+  using Rows = WarpRows<T, LP>;
   __shared__ __align__(16) float bc[2][kScanTile][2][NP];
+  __shared__ __align__(16) T rows[kScanThreads / 32][2][A][K][Rows::kCols];
+  __shared__ __align__(16) T results[kScanThreads / 32][K][Rows::kCols];
   const uint32_t N = a.states;
   const ScanLane<NS, LP> me(a.channels, a.groups, p.per_group, blockIdx.x % p.ctiles);
-  const uint32_t part = threadIdx.x % LP;
+  const uint32_t part = threadIdx.x % LP, col = threadIdx.x % 32 / LP;
   const int64_t chunk = blockIdx.x / p.ctiles;
   const int64_t t0 = chunk * (int64_t)p.len, t1 = min(t0 + (int64_t)p.len, (int64_t)a.seq.tokens);
   f32x2 h[NS / 2], a2[NS / 2];
@@ -219,10 +190,6 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArg
   if (p.carry) load_pairs<NS, FULL>(w.state + row, me.n0, N, h);
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
   const float dskip = a.d ? a.d[me.c] : 0.f;
-  const T* x = reinterpret_cast<const T*>(a.x) + me.c;
-  const T* dt = reinterpret_cast<const T*>(a.dt) + me.c;
-  const T* z = GATE ? reinterpret_cast<const T*>(a.z) + me.c : nullptr;
-  T* y = reinterpret_cast<T*>(a.y) + me.c;
 
   const auto begin_state = [&](int64_t seq) {
     zero_pairs(h);
@@ -239,7 +206,7 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArg
       store_pairs<NS, FULL>(a.final_state + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, h);
   };
   const auto mark = [&](int64_t t) {
-    if (a.marks && t % kMarkEvery == 0 && me.valid)
+    if (a.marks && me.valid)
       store_pairs<NS, FULL>(a.marks + ((uint64_t)(t / kMarkEvery) * a.channels + me.c) * N, me.n0, N, h);
   };
   const auto finish = [&](float o, float xv, float zv) {
@@ -247,85 +214,80 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArg
     if (GATE) o *= zv * sigmoid(zv);
     return from_f32<T>(o);
   };
-  // Whether the tokens of a batch run straight through.
-  constexpr uint32_t kFull = (1u << kAhead) - 1;
-  const auto straight = [](uint32_t live, uint32_t start, uint32_t end) {
-    return (live & kFull) == kFull && !(start & kFull & ~1u) && !(end & (kFull >> 1));
-  };
+  constexpr uint32_t kAll = (1u << K) - 1;
 
+  RowsIn arrays[A];
+  arrays[0] = {a.x, a.x_row};
+  arrays[1] = {a.dt, a.dt_row};
+  if constexpr (GATE) arrays[2] = {a.z, a.z_row};
+  T(*const stages)[A][K][Rows::kCols] = rows[threadIdx.x / 32];
+  T(&result)[K][Rows::kCols] = results[threadIdx.x / 32];
+  const auto fetch = [&](int at, int64_t t, uint32_t live) {
+    Rows::in(stages[at], arrays, t, live, me.warp_c, me.warp_cols, aligned);
+    copies_issued();
+  };
   StageBC<T, NP, 2> stage;
-  Batch<T, LP> now, next;
   TileMarks m = tile_marks(a.seq, t0, t1), after;
   stage.fetch(a, me.group, t0, m.live);
+  fetch(0, t0, m.live);
   stage.put(&bc[0][0][0][0]);
-  const T* px = x + (uint64_t)(t0 + part) * a.x_stride;
-  const T* pdt = dt + (uint64_t)(t0 + part) * a.dt_stride;
-  const T* pz = GATE ? z + (uint64_t)(t0 + part) * a.z_stride : nullptr;
-  T* py = y + (uint64_t)(t0 + part) * a.y_stride;
-  if ((m.live & kFull) == kFull) next.template load<GATE>(px, pdt, pz, a);
   __syncthreads();
-  int buf = 0;
+  int buf = 0, at = 0;
   for (int64_t tb = t0; tb < t1; tb += kScanTile, buf ^= 1, m = after) {
     after = tile_marks(a.seq, tb + kScanTile, t1);
     stage.fetch(a, me.group, tb + kScanTile, after.live);
 #pragma unroll 1
-    for (int k0 = 0; k0 < kScanTile; k0 += kAhead) {
-      const uint32_t live = m.live >> k0, start = m.start >> k0, end = m.end >> k0;
-      now = next;
-      px += kAhead * a.x_stride;
-      pdt += kAhead * a.dt_stride;
-      if (GATE) pz += kAhead * a.z_stride;
-      if (((k0 + kAhead < kScanTile ? m.live >> (k0 + kAhead) : after.live) & kFull) == kFull) next.template load<GATE>(px, pdt, pz, a);
-      if (straight(live, start, end)) {
+    for (int k0 = 0; k0 < kScanTile; k0 += K, at ^= 1) {
+      const uint32_t live = m.live >> k0 & kAll, start = m.start >> k0 & kAll, end = m.end >> k0 & kAll;
+      copies_done();
+      fetch(at ^ 1, tb + k0 + K, k0 + K < kScanTile ? m.live >> (k0 + K) : after.live);
+      const T(&in)[A][K][Rows::kCols] = stages[at];
+      if (live == kAll && !(start & ~1u) && !(end & (kAll >> 1))) {
         if (start & 1) begin_state(tile_seq(m, k0));
         mark(tb + k0);
-        T* to = py;
-        float s[Batch<T, LP>::kOwn], sx[Batch<T, LP>::kOwn], xv[Batch<T, LP>::kOwn], o[LP];
+        float s[kOwn], sx[kOwn], xv[kOwn], o[LP];
 #pragma unroll
-        for (int j = 0; j < Batch<T, LP>::kOwn; ++j) {
-          xv[j] = to_f32(now.x[j]);
-          s[j] = to_f32(now.dt[j]) + bias;
+        for (int j = 0; j < kOwn; ++j) {
+          xv[j] = to_f32(in[0][j * LP + part][col]);
+          s[j] = to_f32(in[1][j * LP + part][col]) + bias;
           if (a.softplus) s[j] = softplus(s[j]);
           sx[j] = s[j] * xv[j];
         }
         f32x2 e[NS / 2], en[NS / 2];
         decay<NS>(from_lane<LP>(s[0], 0), a2, e);
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {  // a token's exponentials are under way while the one before it is added
+        for (int k = 0; k < K; ++k) {  // a token's exponentials are under way while the one before it is added
           const int j = k / LP, q = k % LP;
-          if (k + 1 < kAhead) decay<NS>(from_lane<LP>(s[(k + 1) / LP], (k + 1) % LP), a2, en);
-          const float(&row)[2][NP] = bc[buf][k0 + k];
-          advance<NS, FULL>(e, from_lane<LP>(sx[j], q), &row[0][me.n0], me.n0, N, h);
-          o[q] = dot<NS>(&row[1][me.n0], h);
-          if (q == LP - 1) {
-            const T out = finish(scatter_sum<LP>(o, part), xv[j], GATE ? to_f32(now.z[j]) : 0.f);
-            if (me.valid) *to = out;
-            to += LP * a.y_stride;
-          }
+          if (k + 1 < K) decay<NS>(from_lane<LP>(s[(k + 1) / LP], (k + 1) % LP), a2, en);
+          const float(&bk)[2][NP] = bc[buf][k0 + k];
+          advance<NS, FULL>(e, from_lane<LP>(sx[j], q), &bk[0][me.n0], me.n0, N, h);
+          o[q] = dot<NS>(&bk[1][me.n0], h);
+          if (q == LP - 1)
+            result[j * LP + part][col] = finish(scatter_sum<LP>(o, part), xv[j], GATE ? to_f32(in[A - 1][j * LP + part][col]) : 0.f);
 #pragma unroll
           for (int i = 0; i < NS / 2; ++i) e[i] = en[i];
         }
-        if (end >> (kAhead - 1) & 1) end_state(tile_seq(m, k0 + kAhead - 1));
-      } else if (live & kFull) {
+        if (end >> (K - 1) & 1) end_state(tile_seq(m, k0 + K - 1));
+      } else if (live) {
 #pragma unroll 1
-        for (int k = 0; k < kAhead; ++k) {
+        for (int k = 0; k < K; ++k) {
           if (!(live >> k & 1)) continue;
           if (start >> k & 1) begin_state(tile_seq(m, k0 + k));
-          const uint64_t t = (uint64_t)(tb + k0 + k);
-          mark((int64_t)t);
-          const float xv = to_f32(x[t * a.x_stride]);
-          float s = to_f32(dt[t * a.dt_stride]) + bias;
+          if (k == 0) mark(tb + k0);
+          const float xv = to_f32(in[0][k][col]);
+          float s = to_f32(in[1][k][col]) + bias;
           if (a.softplus) s = softplus(s);
-          const float(&row)[2][NP] = bc[buf][k0 + k];
+          const float(&bk)[2][NP] = bc[buf][k0 + k];
           f32x2 e[NS / 2];
           decay<NS>(s, a2, e);
-          advance<NS, FULL>(e, s * xv, &row[0][me.n0], me.n0, N, h);
-          const T out = finish(sum_lanes<LP>(dot<NS>(&row[1][me.n0], h)), xv, GATE ? to_f32(z[t * a.z_stride]) : 0.f);
-          if (me.valid && me.first) y[t * a.y_stride] = out;
+          advance<NS, FULL>(e, s * xv, &bk[0][me.n0], me.n0, N, h);
+          const float o = sum_lanes<LP>(dot<NS>(&bk[1][me.n0], h));
+          if (me.first) result[k][col] = finish(o, xv, GATE ? to_f32(in[A - 1][k][col]) : 0.f);
           if (end >> k & 1) end_state(tile_seq(m, k0 + k));
         }
       }
-      py += kAhead * a.y_stride;
+      __syncwarp();
+      Rows::out(result, a.y, a.y_row, tb + k0, live, me.warp_c, me.warp_cols, aligned);
     }
     stage.put(&bc[buf ^ 1][0][0][0]);
     __syncthreads();
@@ -406,13 +368,14 @@ cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
   if (a.state != a.final_state || !a.state) w.start = nullptr;
   const uint64_t grid = p.chunks * p.ctiles;
   if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
+  const bool aligned = rows_aligned<T, LP>(a, {{a.x, a.x_row}, {a.dt, a.dt_row}, {a.z, a.z_row}, {a.y, a.y_row}});
   if (p.carry) {
-    sscan_chunk_kernel<T, NS, LP, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w);
+    sscan_chunk_kernel<T, NS, LP, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w, aligned);
     const uint64_t cells = (uint64_t)a.channels * a.states;
     sscan_fold_kernel<false><<<(unsigned)((cells + 255) / 256), 256, 0, s>>>(a.a, w, p.chunks, a.channels, a.states);
   }
-  if (a.z) sscan_kernel<T, NS, LP, FULL, true><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w);
-  else sscan_kernel<T, NS, LP, FULL, false><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w);
+  if (a.z) sscan_kernel<T, NS, LP, FULL, true><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w, aligned);
+  else sscan_kernel<T, NS, LP, FULL, false><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w, aligned);
   return cudaGetLastError();
 }
 

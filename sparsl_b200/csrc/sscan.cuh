@@ -3,6 +3,8 @@
 // arithmetic.
 #pragma once
 
+#include <initializer_list>
+
 #include "seq.cuh"
 
 namespace sparsl {
@@ -89,8 +91,7 @@ inline uint64_t scan_work(const ScanPlan& p, uint32_t channels, uint32_t states,
 // log(1 + e^v): max(v, 0) + log1p(u) with u = e^-|v| in [0, 1], log1p(u) / u by
 // its degree-9 Chebyshev interpolant there (relative error 1e-7 in f32, small
 // steps included).
-__device__ __forceinline__ float softplus(float v) {
-  const float u = ex2(-kLog2e * fabsf(v));
+__device__ __forceinline__ float softplus_from(float v, float u) {
   float p = -0.0031760570127516985f;
   p = __fmaf_rn(p, u, 0.019542526453733444f);
   p = __fmaf_rn(p, u, -0.056373611092567444f);
@@ -102,6 +103,21 @@ __device__ __forceinline__ float softplus(float v) {
   p = __fmaf_rn(p, u, -0.49999892711639404f);
   p = __fmaf_rn(p, u, 1.0f);
   return __fmaf_rn(u, p, fmaxf(v, 0.0f));
+}
+__device__ __forceinline__ float softplus(float v) { return softplus_from(v, ex2(-kLog2e * fabsf(v))); }
+
+// The same and its slope, the sigmoid of v, from one exponential.
+__device__ __forceinline__ float softplus(float v, float& slope) {
+  const float u = ex2(-kLog2e * fabsf(v)), r = rcp(1.0f + u);
+  slope = v >= 0.0f ? r : u * r;
+  return softplus_from(v, u);
+}
+
+// A channel's value in row t of a token array.
+template <class T>
+__device__ __forceinline__ T* cell(const void* p, int64_t t, uint32_t row, uint32_t c) {
+  const char* q = static_cast<const char*>(p) + ((uint64_t)(uint32_t)t * row + c * (uint32_t)sizeof(T));
+  return reinterpret_cast<T*>(const_cast<char*>(q));
 }
 
 // NS states of a channel, from index n0 of N; FULL: all exist and every row is
@@ -174,6 +190,7 @@ __device__ __forceinline__ int64_t tile_seq(const TileMarks& m, int k) {
 template <int NS, int LP>
 struct ScanLane {
   uint32_t group, c, n0, channel_tile, first;
+  uint32_t warp_c, warp_cols;  // the warp's first channel, and how many it has
   bool valid;  // the lane's channel exists (else it works on the group's last one and writes nothing)
   __device__ __forceinline__ ScanLane(uint32_t channels, uint32_t groups, uint32_t per_group, uint32_t ct) {
     constexpr uint32_t kWarp = 32 / LP, kBlock = kScanThreads / LP;
@@ -184,6 +201,9 @@ struct ScanLane {
     const uint32_t cl = channel_tile * kBlock + warp * kWarp + lane / LP;
     valid = cl < cpg;
     c = group * cpg + (valid ? cl : cpg - 1);
+    const uint32_t w0 = channel_tile * kBlock + warp * kWarp;
+    warp_c = group * cpg + (w0 < cpg ? w0 : cpg - 1);
+    warp_cols = w0 >= cpg ? 0 : cpg - w0 < kWarp ? cpg - w0 : kWarp;
     n0 = (lane % LP) * NS;
     first = lane % LP == 0;
   }
@@ -274,5 +294,96 @@ __device__ __forceinline__ float scatter_sum(float (&o)[LP], uint32_t part) {
 }
 
 __device__ __forceinline__ uint32_t first_bits(int64_t n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
+
+// A batch of eight tokens: its rows are copied into shared memory, a warp's
+// channels by that warp, while the batch before it is computed, and its results
+// leave together.  The copies are asynchronous where every piece of a row is
+// aligned: loads into registers would be waited for at the first shared-memory
+// load behind them, since a warp has few scoreboards for both.
+constexpr int kBatch = 8;
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from, uint32_t bytes) {
+  const uint32_t s = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(from), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(s), "l"(from), "n"(BYTES), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_done() {
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
+}
+
+struct RowsIn {
+  const void* p;
+  uint32_t row;  // bytes
+};
+
+template <class T, int LP>
+struct WarpRows {
+  static constexpr int kCols = 32 / LP, kBytes = kCols * (int)sizeof(T), kPiece = kBytes < 16 ? kBytes : 16, kPieces = kBytes / kPiece;
+  static constexpr int kLanes = kBatch * kPieces;  // pieces of one array's batch
+  // Rows t.. of the arrays, from channel c0 on, `cols` of them, those that
+  // `live` names; PER pieces of the A arrays' batches for each lane.
+  template <int A>
+  static __device__ __forceinline__ void in(T (*to)[kBatch][kCols], const RowsIn (&from)[A], int64_t t, uint32_t live,
+                                            uint32_t c0, uint32_t cols, bool aligned) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (aligned) {
+#pragma unroll
+      for (int it = 0; it < (A * kLanes + 31) / 32; ++it) {
+        const uint32_t i = it * 32 + lane, piece = i % kPieces, k = i / kPieces % kBatch, which = i / kLanes;
+        if (which >= A || !(live >> k & 1)) continue;
+        RowsIn r = from[0];
+#pragma unroll
+        for (int q = 1; q < A; ++q)
+          if (which == (uint32_t)q) r = from[q];
+        const uint32_t first = piece * kPiece, have = cols * (uint32_t)sizeof(T);
+        if (have <= first) continue;
+        copy_async<kPiece>(reinterpret_cast<char*>(&to[which][k][0]) + first,
+                           reinterpret_cast<const char*>(cell<T>(r.p, t + k, r.row, c0)) + first,
+                           have - first < kPiece ? have - first : kPiece);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < A; ++q)
+#pragma unroll
+        for (int it = 0; it < kBatch / LP; ++it) {
+          const uint32_t k = it * LP + lane / kCols, c = lane % kCols;
+          if ((live >> k & 1) && c < cols) to[q][k][c] = *cell<T>(from[q].p, t + k, from[q].row, c0 + c);
+        }
+    }
+  }
+  // The batch's results: rows t.. of one array.
+  static __device__ __forceinline__ void out(const T (&from)[kBatch][kCols], void* to, uint32_t row, int64_t t, uint32_t live,
+                                             uint32_t c0, uint32_t cols, bool aligned) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (aligned && cols == kCols) {
+      using Piece = Pack<T, kPiece / (int)sizeof(T)>;
+#pragma unroll
+      for (int it = 0; it < (kLanes + 31) / 32; ++it) {
+        const uint32_t i = it * 32 + lane, piece = i % kPieces, k = i / kPieces;
+        if (k < kBatch && (live >> k & 1))
+          reinterpret_cast<Piece*>(cell<T>(to, t + k, row, c0))[piece] = reinterpret_cast<const Piece*>(&from[k][0])[piece];
+      }
+    } else {
+#pragma unroll
+      for (int it = 0; it < kBatch / LP; ++it) {
+        const uint32_t k = it * LP + lane / kCols, c = lane % kCols;
+        if ((live >> k & 1) && c < cols) *cell<T>(to, t + k, row, c0 + c) = from[k][c];
+      }
+    }
+  }
+};
+// Whether the pieces of a warp's channels start on their own size in every row.
+template <class T, int LP>
+bool rows_aligned(const SscanArgs& a, std::initializer_list<RowsIn> rows) {
+  uint64_t bits = (uint64_t)(a.groups > 1 ? a.channels / a.groups : 0) * sizeof(T);
+  for (const RowsIn& r : rows)
+    if (r.p) bits |= reinterpret_cast<uint64_t>(r.p) | (a.seq.tokens > 1 ? r.row : 0);
+  return bits % WarpRows<T, LP>::kPiece == 0;
+}
 
 }  // namespace sparsl

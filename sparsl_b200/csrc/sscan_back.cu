@@ -6,14 +6,17 @@
 //   dA = sum_t g e h_{t-1} s      dB = sum_c g s x       dC = sum_c dy h
 //
 // The forward pass saved the states before every kMarkEvery-th token.  A block
-// of that many tokens is recomputed forwards from its mark with the decays and
-// states kept in registers, and then walked backwards, so each exponential is
-// computed once.  Chunks of the token axis run in parallel as in the forward
+// of that many tokens is recomputed forwards from its mark with the states kept
+// in registers, and then walked backwards.  Its decays are computed once more
+// on the way back: the special function unit has the time, the registers to
+// keep them hold the next block's rows instead.  Chunks of the token axis run in parallel as in the forward
 // pass: the gradient each chunk hands to the one before it is computed first,
 // and folded.  dB and dC are summed over a warp's channels and a block's warps
 // in shared memory, and over the blocks' partial rows in a fixed order, so that
 // results do not change from run to run; so are dA, dD and the step bias's
 // gradient over the chunks.
+#include <type_traits>
+
 #include "sscan.cuh"
 
 namespace sparsl {
@@ -24,7 +27,8 @@ cudaError_t launch_sscan_fold_back(const float* a, const ScanWork& w, uint64_t c
 namespace {
 
 constexpr int kWarps = kScanThreads / 32;
-constexpr uint32_t kResident = 2;  // blocks an SM holds, at up to 255 registers a thread
+// Blocks an SM holds: at 128 registers a thread with 4 states, 255 with 8.
+constexpr int resident(int states) { return states == 4 ? 4 : 2; }
 constexpr int kBlock = (int)kMarkEvery;
 
 struct BackWork {
@@ -136,24 +140,26 @@ __global__ void __launch_bounds__(kScanThreads, 4) sscan_chunk_back_kernel(Sscan
 }
 
 // Sums over a warp's channels.  For each of four tokens a warp's lanes leave
-// 8 states each in 1 KB of shared memory: row by row of channels, a row's
-// quads of states at slot ^ turn(row), which keeps both the lanes' stores (a
-// row after another) and the sums' loads (a slot's quads of several rows) on
-// different banks.  Adding in shared memory takes a fifth of the instructions
-// of exchanges between lanes.
-template <int LP>
+// their states in 128 NS bytes of shared memory: row by row of channels, quads
+// of states at slot ^ turn(row), so that neither the lanes' stores (a row after
+// another) nor the sums' loads (a slot's quads of several rows) meet on a bank.
+// Adding in shared memory takes a fraction of the instructions that exchanges
+// between lanes take.
+template <int NS, int LP>
 struct WarpSum {
-  static constexpr int kRows = 32 / LP, kSlots = 2 * LP, kShare = LP <= 4 ? 4 / LP : 1;  // lanes per sum
+  static constexpr int kRows = 32 / LP, kEach = NS / 4, kSlots = kEach * LP, kQuads = 8 * NS;  // kQuads: of a token
+  static constexpr int kShare = 32 / (4 * kSlots) > 0 ? 32 / (4 * kSlots) : 1;                 // lanes per sum
   static constexpr int kItems = 4 * kSlots * kShare;
   static __device__ __forceinline__ uint32_t turn(uint32_t row) {
-    return LP <= 4 ? (row >> (LP == 1 ? 2 : LP == 2 ? 1 : 0) & 1) * LP : 0;
+    if constexpr (NS == 4 || LP > 4) return 0;
+    else return (row >> (LP == 1 ? 2 : LP == 2 ? 1 : 0) & 1) * LP;
   }
-  // Lane's states 0..7 of token k (0..3).
-  static __device__ __forceinline__ void put(float* v, int k, const f32x2 (&s)[4]) {
+  // Lane's states of token k (0..3).
+  static __device__ __forceinline__ void put(float* v, int k, const f32x2 (&s)[NS / 2]) {
     const uint32_t lane = threadIdx.x & 31, row = lane / LP, part = lane % LP;
-    ulonglong2* q = reinterpret_cast<ulonglong2*>(v) + k * 64 + row * kSlots;
-    q[part ^ turn(row)] = make_ulonglong2(s[0], s[1]);
-    q[(LP + part) ^ turn(row)] = make_ulonglong2(s[2], s[3]);
+    ulonglong2* q = reinterpret_cast<ulonglong2*>(v) + k * kQuads + row * kSlots;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) q[(i * LP + part) ^ turn(row)] = make_ulonglong2(s[2 * i], s[2 * i + 1]);
   }
   // The four tokens' sums to out[token * stride + state].
   static __device__ __forceinline__ void add(const float* v, float* out, int stride) {
@@ -162,14 +168,14 @@ struct WarpSum {
 #pragma unroll
     for (int it = 0; it < kItems / 32; ++it) {
       const uint32_t item = it * 32 + lane, k = item / (kSlots * kShare), slot = item / kShare % kSlots, share = item % kShare;
-      const ulonglong2* q = reinterpret_cast<const ulonglong2*>(v) + k * 64;
+      const ulonglong2* q = reinterpret_cast<const ulonglong2*>(v) + k * kQuads;
       f32x2 lo = 0ull, hi = 0ull;
 #pragma unroll
       for (int i = 0; i < kRows / kShare; ++i) {
         const uint32_t row = i * kShare + share;
         const ulonglong2 t = q[row * kSlots + (slot ^ turn(row))];
-        lo = add2(lo, t.x);
-        hi = add2(hi, t.y);
+        lo = i ? add2(lo, t.x) : t.x;
+        hi = i ? add2(hi, t.y) : t.y;
       }
       float s[4];
       unpair(lo, s[0], s[1]);
@@ -179,33 +185,37 @@ struct WarpSum {
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
       if (share == 0)
-        *reinterpret_cast<float4*>(out + k * stride + slot % LP * 8 + slot / LP * 4) = make_float4(s[0], s[1], s[2], s[3]);
+        *reinterpret_cast<float4*>(out + k * stride + slot % LP * NS + slot / LP * 4) = make_float4(s[0], s[1], s[2], s[3]);
     }
     __syncwarp();
   }
 };
 
-template <int NP>
+template <int NS, int LP>
 struct BackShared {
-  float bc[2][kScanTile][2][NP];
-  float red[2][kWarps][2][kBlock][NP];  // dB's sums, then dC's
-  float sum[kWarps][4][256];
+  float bc[2][kScanTile][2][NS * LP];
+  float red[2][kWarps][2][kBlock][NS * LP];  // dB's sums, then dC's
+  float sum[kWarps][4][32 * NS];
+  float4 cell[kWarps][kBlock][32 / LP];  // step, step times x, gradient behind the gate
 };
 
 // A block of kBlock tokens at a time, last ones first: forwards from its mark
-// with decays and states kept in registers, then backwards.
-template <class T, int LP, bool FULL, bool GATE>
-__global__ void __launch_bounds__(kScanThreads, kResident) sscan_back_kernel(SscanArgs a, ScanPlan p, BackWork w) {
-  constexpr int NS = 8, NP = NS * LP, K = kBlock, kOwn = K / LP;
+// with the states kept in registers, then backwards.  EDGES: a sequence begins
+// or ends inside the block.
+template <class T, int NS, int LP, bool FULL, bool GATE>
+__global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(SscanArgs a, ScanPlan p, BackWork w) {
+  constexpr int NP = NS * LP, NH = NS / 2, K = kBlock, kOwn = K / LP, kEach = K * 2 * NP / kScanThreads;
   extern __shared__ __align__(16) unsigned char shared_bytes[];
-  BackShared<NP>& sh = *reinterpret_cast<BackShared<NP>*>(shared_bytes);
+  BackShared<NS, LP>& sh = *reinterpret_cast<BackShared<NS, LP>*>(shared_bytes);
   const uint32_t N = a.states;
   const ScanLane<NS, LP> me(a.channels, a.groups, p.per_group, blockIdx.x % p.ctiles);
   const uint32_t part = threadIdx.x % LP, warp = threadIdx.x >> 5;
   const int64_t chunk = blockIdx.x / p.ctiles;
   const int64_t t0 = chunk * (int64_t)p.len, t1 = min(t0 + (int64_t)p.len, (int64_t)a.seq.tokens);
   float* sums = &sh.sum[warp][0][0];
-  f32x2 a2[4], r[4], da[4];
+  constexpr int kRows = 32 / LP;
+  float4* const cells = &sh.cell[warp][0][threadIdx.x % 32 / LP];  // this channel's, of the block's tokens
+  f32x2 a2[NH], r[NH], da[NH];
   load_pairs<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2, kLog2e);
   zero_pairs(r);
   zero_pairs(da);
@@ -214,26 +224,28 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_back_kernel(Ssc
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
   const float dskip = a.d ? a.d[me.c] : 0.f;
   float dd = 0.f, dbias = 0.f;
-  T xr[kOwn], dr[kOwn], gr[kOwn], zr[kOwn];
-  // Own tokens of the block from t on that `live` names.
-  const auto load = [&](int64_t t, uint32_t live) {
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-      if (!(live >> (j * LP + part) & 1)) continue;
-      const uint64_t at = (uint64_t)t + j * LP + part;
-      xr[j] = reinterpret_cast<const T*>(a.x)[at * a.x_stride + me.c];
-      dr[j] = reinterpret_cast<const T*>(a.dt)[at * a.dt_stride + me.c];
-      gr[j] = reinterpret_cast<const T*>(a.dy)[at * a.dy_stride + me.c];
-      if (GATE) zr[j] = reinterpret_cast<const T*>(a.z)[at * a.z_stride + me.c];
-    }
-  };
-  const auto mark_of = [&](int64_t t) {
-    return a.marks + ((uint64_t)(t / K) * a.channels + me.c) * N;
-  };
   const auto state_row = [&](int64_t seq) {
     const int64_t slot = a.seq.slot(seq);
     return slot < 0 || !me.valid ? -1 : (int64_t)(((uint64_t)slot * a.channels + me.c) * N);
   };
+  // Own tokens of the block from t on that `live` names, and the state at its mark.
+  T xr[kOwn], dr[kOwn], gr[kOwn], zr[kOwn];
+  f32x2 marked[NH];
+  const auto fetch = [&](int64_t t, uint32_t live) {
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j)
+      if (live >> (j * LP + part) & 1) {
+        const int64_t at = t + j * LP + part;
+        xr[j] = *cell<T>(a.x, at, a.x_row, me.c);
+        dr[j] = *cell<T>(a.dt, at, a.dt_row, me.c);
+        gr[j] = *cell<T>(a.dy, at, a.dy_row, me.c);
+        if (GATE) zr[j] = *cell<T>(a.z, at, a.z_row, me.c);
+      }
+    if (live & 1) load_pairs<NS, FULL>(a.marks + ((uint64_t)(t / K) * a.channels + me.c) * N, me.n0, N, marked);
+  };
+  // Where this thread puts its sums over the block's warps: row t of its channel tile, its own offsets in there.
+  float* const part_rows = w.bc + ((uint64_t)me.channel_tile * a.seq.tokens * a.groups + me.group) * 2 * N;
+  const uint32_t part_row = a.groups * 2 * N;
 
   const int64_t tiles = (t1 - t0 + kScanTile - 1) / kScanTile;
   StageBC<T, NP, 2> stage;
@@ -242,7 +254,7 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_back_kernel(Ssc
     m = tile_marks(a.seq, t0 + (tiles - 1) * kScanTile, t1);
     stage.fetch(a, me.group, t0 + (tiles - 1) * kScanTile, m.live);
     stage.put(&sh.bc[0][0][0][0]);
-    load(t0 + tiles * kScanTile - K, m.live >> (kScanTile - K));
+    fetch(t0 + tiles * kScanTile - K, m.live >> (kScanTile - K));
   }
   __syncthreads();
   int buf = 0, out = 0;
@@ -255,22 +267,20 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_back_kernel(Ssc
     }
 #pragma unroll 1
     for (int k0 = kScanTile - K; k0 >= 0; k0 -= K) {
-      const uint32_t live = m.live >> k0 & ((1u << K) - 1), start = m.start >> k0, end = m.end >> k0;
-      const uint32_t live_next = k0 ? m.live >> (k0 - K) : before.live >> (kScanTile - K);
+      constexpr uint32_t kAll = (1u << K) - 1;
+      const uint32_t live = m.live >> k0 & kAll, start = m.start >> k0 & kAll, end = m.end >> k0 & kAll;
+      const int64_t tk = tb + k0;
       // This lane's own tokens: steps, gates; those that are no tokens change nothing (e = 1).
-      float s[kOwn], sx[kOwn], g[kOwn], xv[kOwn], slope[kOwn], gg[kOwn];
+      float s[kOwn], g[kOwn], xv[kOwn], slope[kOwn], gg[kOwn];
+      __syncwarp();
 #pragma unroll
       for (int j = 0; j < kOwn; ++j) {
-        s[j] = sx[j] = g[j] = xv[j] = slope[j] = gg[j] = 0.f;
+        s[j] = g[j] = xv[j] = slope[j] = gg[j] = 0.f;
         if ((live >> (j * LP + part) & 1) && me.valid) {
           xv[j] = to_f32(xr[j]);
           s[j] = to_f32(dr[j]) + bias;
           slope[j] = 1.f;
-          if (a.softplus) {
-            slope[j] = sigmoid(s[j]);
-            s[j] = softplus(s[j]);
-          }
-          sx[j] = s[j] * xv[j];
+          if (a.softplus) s[j] = softplus(s[j], slope[j]);
           g[j] = to_f32(gr[j]);
           if (GATE) {
             const float zv = to_f32(zr[j]), sig = sigmoid(zv);
@@ -278,29 +288,41 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_back_kernel(Ssc
             g[j] *= zv * sig;
           }
         }
+        cells[(j * LP + part) * kRows] = make_float4(s[j], s[j] * xv[j], g[j], 0.f);
       }
-      f32x2 h[4], hp[K][4], e[K][4];
+      __syncwarp();
+      f32x2 h[NH];
       zero_pairs(h);
-      if ((live & 1) && me.valid) load_pairs<NS, FULL>(mark_of(tb + k0), me.n0, N, h);
-      load(tb + k0 - K, live_next);
-      if (live) {
-        // Forwards.
+      if ((live & 1) && me.valid)
+#pragma unroll
+        for (int i = 0; i < NH; ++i) h[i] = marked[i];
+      fetch(tk - K, k0 ? m.live >> (k0 - K) : before.live >> (kScanTile - K));
+      const float(*const rows)[2][NP] = &sh.bc[buf][k0];
+      float(*const red)[K][NP] = sh.red[out][warp];
+      const auto walk = [&](auto edges) {
+        constexpr bool EDGES = decltype(edges)::value;
+        f32x2 hp[K][NH], e[NH], en[NH];
         float o[LP];
+        // Forwards.
+        float4 now = cells[0], next;
+        decay<NS>(now.x, a2, e);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const int j = k / LP, q = k % LP;
-          if (k && (start >> k & 1)) {
+          if (k + 1 < K) {
+            next = cells[(k + 1) * kRows];
+            decay<NS>(next.x, a2, en);
+          }
+          if (EDGES && k && (start >> k & 1)) {
             zero_pairs(h);
             const int64_t at = a.state ? state_row(tile_seq(m, k0 + k)) : -1;
             if (at >= 0) load_pairs<NS, FULL>(a.state + at, me.n0, N, h);
           }
-          decay<NS>(from_lane<LP>(s[j], q), a2, e[k]);
-          const float xq = from_lane<LP>(sx[j], q), gq = from_lane<LP>(g[j], q);
-          const f32x2 xx = pair(xq, xq), gv = pair(gq, gq);
-          f32x2 v[4], oo = 0ull;
+          const f32x2 xx = pair(now.y, now.y), gv = pair(now.z, now.z);
+          f32x2 v[NH], oo = 0ull;
 #pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sh.bc[buf][k0 + k][0][me.n0 + 2 * i]);
+          for (int i = 0; i < NH; i += 2) {
+            const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&rows[k][0][me.n0 + 2 * i]);
             f32x2 add[2] = {mul2(xx, bb.x), mul2(xx, bb.y)};
             if (!FULL) {
 #pragma unroll
@@ -314,56 +336,64 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_back_kernel(Ssc
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               hp[k][i + u] = h[i + u];
-              h[i + u] = fma2(e[k][i + u], h[i + u], add[u]);
+              h[i + u] = fma2(e[i + u], h[i + u], add[u]);
               v[i + u] = mul2(gv, h[i + u]);
             }
             if (GATE) {
-              const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sh.bc[buf][k0 + k][1][me.n0 + 2 * i]);
+              const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&rows[k][1][me.n0 + 2 * i]);
               oo = fma2(cc.x, h[i], oo);
               oo = fma2(cc.y, h[i + 1], oo);
             }
           }
-          WarpSum<LP>::put(sums, k & 3, v);
-          if ((k & 3) == 3) WarpSum<LP>::add(sums, &sh.red[out][warp][1][k - 3][0], NP);
+          WarpSum<NS, LP>::put(sums, k & 3, v);
+          if ((k & 3) == 3) WarpSum<NS, LP>::add(sums, &red[1][0][0] + (k - 3) * NP, NP);
           if (GATE) {
             o[q] = sum2(oo);
             if (q == LP - 1) {
               const float pre = __fmaf_rn(dskip, xv[j], scatter_sum<LP>(o, part));
               if ((live >> (j * LP + part) & 1) && me.valid)
-                reinterpret_cast<T*>(a.dz)[(uint64_t)(tb + k0 + j * LP + part) * a.dz_stride + me.c] = from_f32<T>(gg[j] * pre);
+                *cell<T>(a.dz, tk + j * LP + part, a.dz_row, me.c) = from_f32<T>(gg[j] * pre);
             }
           }
+#pragma unroll
+          for (int i = 0; i < NH; ++i) e[i] = en[i];
+          now = next;
         }
         // Backwards.
         float gb[LP], ga[LP];
+        now = cells[(K - 1) * kRows];
+        decay<NS>(now.x, a2, e);
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) {
           const int j = k / LP, q = k % LP;
-          if (end >> k & 1) {
+          if (k) {
+            next = cells[(k - 1) * kRows];
+            decay<NS>(next.x, a2, en);
+          }
+          if ((EDGES || k == K - 1) && (end >> k & 1)) {
             zero_pairs(r);
             const int64_t at = a.dfinal ? state_row(tile_seq(m, k0 + k)) : -1;
             if (at >= 0) load_pairs<NS, FULL>(a.dfinal + at, me.n0, N, r);
           }
-          const float sq = from_lane<LP>(s[j], q), xq = from_lane<LP>(sx[j], q), gq = from_lane<LP>(g[j], q);
-          const f32x2 ss = pair(sq, sq), xx = pair(xq, xq), gv = pair(gq, gq);
-          f32x2 v[4], gb2 = 0ull, ga2 = 0ull;
+          const f32x2 ss = pair(now.x, now.x), xx = pair(now.y, now.y), gv = pair(now.z, now.z);
+          f32x2 v[NH], gb2 = 0ull, ga2 = 0ull;
 #pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&sh.bc[buf][k0 + k][0][me.n0 + 2 * i]);
-            const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&sh.bc[buf][k0 + k][1][me.n0 + 2 * i]);
+          for (int i = 0; i < NH; i += 2) {
+            const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(&rows[k][0][me.n0 + 2 * i]);
+            const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(&rows[k][1][me.n0 + 2 * i]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const f32x2 gh = fma2(u ? cc.y : cc.x, gv, r[i + u]);
               gb2 = fma2(gh, u ? bb.y : bb.x, gb2);
-              r[i + u] = mul2(e[k][i + u], gh);
+              r[i + u] = mul2(e[i + u], gh);
               const f32x2 through = mul2(r[i + u], hp[k][i + u]);
               ga2 = fma2(through, a2[i + u], ga2);
               da[i + u] = fma2(through, ss, da[i + u]);
               v[i + u] = mul2(gh, xx);
             }
           }
-          WarpSum<LP>::put(sums, k & 3, v);
-          if ((k & 3) == 0) WarpSum<LP>::add(sums, &sh.red[out][warp][0][k][0], NP);
+          WarpSum<NS, LP>::put(sums, k & 3, v);
+          if ((k & 3) == 0) WarpSum<NS, LP>::add(sums, &red[0][0][0] + k * NP, NP);
           gb[q] = sum2(gb2);
           ga[q] = sum2(ga2);
           if (q == 0) {
@@ -372,27 +402,33 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_back_kernel(Ssc
               const float ds = __fmaf_rn(gas, 1.0f / kLog2e, xv[j] * gbs) * slope[j];
               dd = __fmaf_rn(g[j], xv[j], dd);
               dbias += ds;
-              const uint64_t t = (uint64_t)(tb + k0 + j * LP + part);
-              reinterpret_cast<T*>(a.dx)[t * a.dx_stride + me.c] = from_f32<T>(__fmaf_rn(dskip, g[j], s[j] * gbs));
-              reinterpret_cast<T*>(a.ddt)[t * a.ddt_stride + me.c] = from_f32<T>(ds);
+              const int64_t t = tk + j * LP + part;
+              *cell<T>(a.dx, t, a.dx_row, me.c) = from_f32<T>(__fmaf_rn(dskip, g[j], s[j] * gbs));
+              *cell<T>(a.ddt, t, a.ddt_row, me.c) = from_f32<T>(ds);
             }
           }
-          if (start >> k & 1) {
+          if ((EDGES || k == 0) && (start >> k & 1)) {
             const int64_t at = a.dstate ? state_row(tile_seq(m, k0 + k)) : -1;
             if (at >= 0) store_pairs<NS, FULL>(a.dstate + at, me.n0, N, r);
             zero_pairs(r);  // rows in front of it belong to no sequence, or end one
           }
+#pragma unroll
+          for (int i = 0; i < NH; ++i) e[i] = en[i];
+          now = next;
         }
-      }
+      };
+      if (live == kAll && !(start & ~1u) && !(end & (kAll >> 1))) walk(std::false_type{});
+      else if (live) walk(std::true_type{});
       __syncthreads();
-      for (int i = threadIdx.x; i < K * 2 * NP; i += kScanThreads) {
-        const uint32_t n = i % NP, k = i / NP % K, which = i / (NP * K);
+      float* const to = part_rows + (uint64_t)(uint32_t)tk * part_row;
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) {
+        const uint32_t i = u * kScanThreads + threadIdx.x, n = i % NP, k = i / NP % K, which = i / (NP * K);
         if (n >= N || !(live >> k & 1)) continue;
         float v = 0.f;
 #pragma unroll
         for (int q = 0; q < kWarps; ++q) v += sh.red[out][q][which][k][n];
-        const uint64_t t = (uint64_t)(tb + k0 + k);
-        w.bc[((((uint64_t)me.channel_tile * a.seq.tokens + t) * a.groups + me.group) * 2 + which) * N + n] = v;
+        to[k * part_row + which * N + n] = v;
       }
       out ^= 1;  // the next block of tokens writes the other one while this is read
     }
@@ -440,11 +476,13 @@ __global__ void __launch_bounds__(256) sscan_bc_kernel(SscanArgs a, const float*
 
 bool aligned16(const void* p) { return reinterpret_cast<uint64_t>(p) % 16 == 0; }
 
-// 8 states a lane: a block of kMarkEvery tokens of them fits the registers.
-constexpr uint32_t lanes_of(uint32_t states) { return states <= 8 ? 1 : states <= 16 ? 2 : states <= 32 ? 4 : 8; }
+// 4 states a lane (16 warps an SM), 8 where there are more than 32: a token's
+// own work can be divided among 8 lanes at most.
+constexpr uint32_t lanes_of(uint32_t states) { return states <= 8 ? 2 : states <= 16 ? 4 : 8; }
 
 ScanPlan plan_of(uint64_t tokens, uint32_t channels, uint32_t states, uint64_t n_seq, uint32_t groups, bool ragged) {
-  return scan_plan(tokens, channels, groups, n_seq, ragged, {lanes_of(states), lanes_of(states), kResident});
+  const uint32_t l = lanes_of(states);
+  return scan_plan(tokens, channels, groups, n_seq, ragged, {l, l, (uint32_t)resident(states <= 32 ? 4 : 8)});
 }
 
 uint64_t back_work(const ScanPlan& p, uint64_t tokens, uint32_t channels, uint32_t states, uint32_t groups, void* base,
@@ -459,7 +497,7 @@ uint64_t back_work(const ScanPlan& p, uint64_t tokens, uint32_t channels, uint32
   return at + scan_round((uint64_t)p.per_group * tokens * groups * 2 * states * 4);
 }
 
-template <class T, int LP, bool FULL, bool GATE>
+template <class T, int NS, int LP, bool FULL, bool GATE>
 cudaError_t go(const SscanArgs& a, cudaStream_t s) {
   const ScanPlan p = plan_of(a.seq.tokens, a.channels, a.states, a.seq.n_seq, a.groups, a.seq.seq_ptr != nullptr);
   BackWork w{};
@@ -469,7 +507,7 @@ cudaError_t go(const SscanArgs& a, cudaStream_t s) {
   cudaError_t e;
   if (p.carry) {
     // The same chunks with up to 16 states a lane: there is no history to keep.
-    constexpr int CL = LP <= 2 ? 1 : LP / 2, CS = LP * 8 / CL;
+    constexpr int CL = NS * LP <= 16 ? 1 : NS * LP / 16, CS = NS * LP / CL;
     ScanPlan q = p;
     const uint32_t cpg = a.channels / a.groups;
     q.lanes = CL;
@@ -479,8 +517,8 @@ cudaError_t go(const SscanArgs& a, cudaStream_t s) {
     e = launch_sscan_fold_back(a.a, w.scan, p.chunks, a.channels, a.states, s);
     if (e != cudaSuccess) return e;
   }
-  constexpr int bytes = sizeof(BackShared<8 * LP>);
-  const auto kernel = sscan_back_kernel<T, LP, FULL, GATE>;
+  constexpr int bytes = sizeof(BackShared<NS, LP>);
+  const auto kernel = sscan_back_kernel<T, NS, LP, FULL, GATE>;
   if (bytes > 48 * 1024) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
@@ -497,22 +535,20 @@ cudaError_t go(const SscanArgs& a, cudaStream_t s) {
   return e;
 }
 
-template <class T, int LP>
+template <class T, int NS, int LP>
 cudaError_t by_form(const SscanArgs& a, cudaStream_t s) {
-  const bool full = a.states == 8 * LP && aligned16(a.a) && aligned16(a.state) && aligned16(a.dstate) && aligned16(a.dfinal) &&
-                    aligned16(a.marks) && aligned16(a.work);
-  if (full) return a.z ? go<T, LP, true, true>(a, s) : go<T, LP, true, false>(a, s);
-  return a.z ? go<T, LP, false, true>(a, s) : go<T, LP, false, false>(a, s);
+  const bool full = a.states == NS * LP && aligned16(a.a) && aligned16(a.state) && aligned16(a.dstate) &&
+                    aligned16(a.dfinal) && aligned16(a.marks) && aligned16(a.work);
+  if (full) return a.z ? go<T, NS, LP, true, true>(a, s) : go<T, NS, LP, true, false>(a, s);
+  return a.z ? go<T, NS, LP, false, true>(a, s) : go<T, NS, LP, false, false>(a, s);
 }
 
 template <class T>
 cudaError_t by_states(const SscanArgs& a, cudaStream_t s) {
-  switch (lanes_of(a.states)) {
-    case 1: return by_form<T, 1>(a, s);
-    case 2: return by_form<T, 2>(a, s);
-    case 4: return by_form<T, 4>(a, s);
-    default: return by_form<T, 8>(a, s);
-  }
+  if (a.states <= 8) return by_form<T, 4, 2>(a, s);
+  if (a.states <= 16) return by_form<T, 4, 4>(a, s);
+  if (a.states <= 32) return by_form<T, 4, 8>(a, s);
+  return by_form<T, 8, 8>(a, s);
 }
 
 }  // namespace
