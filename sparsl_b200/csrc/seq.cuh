@@ -225,6 +225,17 @@ cudaError_t launch_sscan(const SscanArgs& a, cudaStream_t s);
 cudaError_t launch_sscan_backward(const SscanArgs& a, cudaStream_t s);
 cudaError_t launch_sscan_step(const SscanArgs& a, cudaStream_t s);
 
+// By the tokens' type.
+cudaError_t launch_sscan_f32(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_f16(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_bf16(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_step_f32(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_step_f16(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_step_bf16(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_backward_f32(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_backward_f16(const SscanArgs& a, cudaStream_t s);
+cudaError_t launch_sscan_backward_bf16(const SscanArgs& a, cudaStream_t s);
+
 // ---- layer norm (norm.cu) ----
 struct NormArgs {
   int type;
