@@ -11,9 +11,18 @@ namespace sparsl {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kBatch = 8;      // rows in flight per thread
-constexpr int kTile = 32;      // tokens of a forward tile
-constexpr int kTileBack = 64;  // tokens of a backward tile: one partial row of dw, dbias each
+constexpr int kRowsAhead = 8;      // rows in flight per thread, asked for while the batch before is computed
+constexpr int kRowsAheadBack = 4;  // of x and of dy each
+constexpr uint32_t kSms = 148;
+
+// Tokens of a tile: 64 (a partial row of dw and dbias each, in the backward
+// pass), fewer where that leaves SMs with fewer than eight blocks.
+uint32_t tile_of(uint64_t tokens, uint64_t channels, uint32_t per_block) {
+  const uint64_t ctiles = (channels + per_block - 1) / per_block;
+  uint32_t tile = 64;
+  while (tile > 16 && (tokens + tile - 1) / tile * ctiles < 8 * kSms) tile /= 2;
+  return tile;
+}
 
 template <class T, int V, int W>
 struct Taps {
@@ -88,21 +97,21 @@ __device__ __forceinline__ void load_weights(const ConvArgs& a, uint32_t c, floa
 // final states, so that only one thread reads and writes a channel of a state
 // and the pool may be updated in place.
 template <class T, int V, int W, bool SILU>
-__global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs a, uint32_t ctiles) {
+__global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs a, uint32_t ctiles, uint32_t tokens_a_tile) {
   const uint32_t ct = blockIdx.x % ctiles;
   const int64_t tile = blockIdx.x / ctiles;
+  const int64_t tokens = (int64_t)a.seq.tokens, n = (int64_t)a.seq.n_seq;
+  const int64_t t0 = tile * tokens_a_tile;
+  const bool last = t0 + tokens_a_tile >= tokens;
+  const int64_t t1 = last ? tokens : t0 + tokens_a_tile;
+  int64_t i = a.seq.first_from_warp(t0);
   const uint32_t c = (ct * kThreads + threadIdx.x) * V;
   if (c >= a.channels) return;
-  const int64_t tokens = (int64_t)a.seq.tokens, n = (int64_t)a.seq.n_seq;
-  const int64_t t0 = tile * kTile;
-  const bool last = t0 + kTile >= tokens;
-  const int64_t t1 = last ? tokens : t0 + kTile;
   float w[W][V], bias[V];
   load_weights<T, V, W>(a, c, w, bias);
   const T* x = reinterpret_cast<const T*>(a.x) + c;
   T* y = reinterpret_cast<T*>(a.y) + c;
 
-  int64_t i = a.seq.first_from(t0);
   int64_t at = t0;  // tokens before it are done
   // i - 1 continues into the tile when it ends behind t0.
   for (i = i > 0 ? i - 1 : 0; i < n; ++i) {
@@ -114,19 +123,25 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs a, uint32_t cti
     int64_t to = min(end, t1);
     if (mine) to = min(end, max(t1, begin + (W - 1)));
     if (from < to) {
+      Pack<T, V> now[kRowsAhead], next[kRowsAhead];
+      const auto ask = [&](int64_t t) {
+#pragma unroll
+        for (int k = 0; k < kRowsAhead; ++k)
+          if (t + k < to) next[k] = *reinterpret_cast<const Pack<T, V>*>(x + (uint64_t)(t + k) * a.x_stride);
+      };
+      ask(from);
       Taps<T, V, W> win;
       load_taps<T, V, W>(a, i, begin, from, c, win);
-      for (int64_t t = from; t < to; t += kBatch) {
-        Pack<T, V> raw[kBatch];
+      for (int64_t t = from; t < to; t += kRowsAhead) {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-          if (t + k < to) raw[k] = *reinterpret_cast<const Pack<T, V>*>(x + (uint64_t)(t + k) * a.x_stride);
+        for (int k = 0; k < kRowsAhead; ++k) now[k] = next[k];
+        ask(t + kRowsAhead);
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
+        for (int k = 0; k < kRowsAhead; ++k) {
           if (t + k >= to) break;
           float v[V], u[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) v[j] = to_f32(raw[k].v[j]);
+          for (int j = 0; j < V; ++j) v[j] = to_f32(now[k].v[j]);
           win.push(v);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
@@ -150,29 +165,29 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs a, uint32_t cti
 // du[t] is.  Positions in front of the sequence are its state's rows, so dstate
 // and the gradient of the final state come out of the same walk.
 template <class T, int V, int W, bool SILU>
-__global__ void __launch_bounds__(kThreads) conv_backward_kernel(ConvArgs a, uint32_t ctiles) {
+__global__ void __launch_bounds__(kThreads) conv_backward_kernel(ConvArgs a, uint32_t ctiles, uint32_t tokens_a_tile) {
   const uint32_t ct = blockIdx.x % ctiles;
   const int64_t tile = blockIdx.x / ctiles;
+  const int64_t tokens = (int64_t)a.seq.tokens, n = (int64_t)a.seq.n_seq;
+  const int64_t t0 = tile * tokens_a_tile;
+  const bool last = t0 + tokens_a_tile >= tokens;
+  const int64_t t1 = last ? tokens : t0 + tokens_a_tile;
+  int64_t i = a.seq.first_from_warp(t0);
   const uint32_t c = (ct * kThreads + threadIdx.x) * V;
   if (c >= a.channels) return;
-  const int64_t tokens = (int64_t)a.seq.tokens, n = (int64_t)a.seq.n_seq;
-  const int64_t t0 = tile * kTileBack;
-  const bool last = t0 + kTileBack >= tokens;
-  const int64_t t1 = last ? tokens : t0 + kTileBack;
   float w[W][V], bias[V], dw[W][V], db[V];
   load_weights<T, V, W>(a, c, w, bias);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    db[i] = 0.f;
+  for (int j = 0; j < V; ++j) {
+    db[j] = 0.f;
 #pragma unroll
-    for (int k = 0; k < W; ++k) dw[k][i] = 0.f;
+    for (int k = 0; k < W; ++k) dw[k][j] = 0.f;
   }
   const T* x = reinterpret_cast<const T*>(a.x) + c;
   const T* dy = reinterpret_cast<const T*>(a.dy) + c;
   T* dx = reinterpret_cast<T*>(a.dx) + c;
 
   int64_t at = t0;
-  int64_t i = a.seq.first_from(t0);
   for (i = i > 0 ? i - 1 : 0; i < n; ++i) {
     const int64_t begin = a.seq.begin(i);
     if (begin >= t1 && !last) break;
@@ -192,52 +207,75 @@ __global__ void __launch_bounds__(kThreads) conv_backward_kernel(ConvArgs a, uin
     const T* df = a.dfinal && slot >= 0 ? reinterpret_cast<const T*>(a.dfinal) + (uint64_t)slot * (W - 1) * a.channels + c
                                         : nullptr;
     T* ds = states && slot >= 0 ? reinterpret_cast<T*>(a.dstate) + (uint64_t)slot * (W - 1) * a.channels + c : nullptr;
-    for (int64_t t = from; t < to + (W - 1); ++t) {
-      float d[V];
+    constexpr int K = kRowsAheadBack;
+    Pack<T, V> xn[K], dn[K], xr[K], dr[K];
+    const int64_t stop = min(to + (W - 1), end);  // tokens behind it have no gradient
+    const auto ask = [&](int64_t t) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = 0.f;
-      if (t < end) {
-        float v[V];
-        load_pack<T, V>(x + (uint64_t)t * a.x_stride, v);
-        load_pack<T, V>(dy + (uint64_t)t * a.dy_stride, d);
-        win.push(v);
-        if (SILU) {
+      for (int k = 0; k < K; ++k)
+        if (t + k < stop) {
+          xn[k] = *reinterpret_cast<const Pack<T, V>*>(x + (uint64_t)(t + k) * a.x_stride);
+          dn[k] = *reinterpret_cast<const Pack<T, V>*>(dy + (uint64_t)(t + k) * a.dy_stride);
+        }
+    };
+    ask(from);
+    for (int64_t tk = from; tk < to + (W - 1); tk += K) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) xr[k] = xn[k], dr[k] = dn[k];
+      ask(tk + K);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int64_t t = tk + k;
+        if (t >= to + (W - 1)) break;
+        float d[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] = 0.f;
+        if (t < end) {
+          float v[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            float u = bias[j];
+            v[j] = to_f32(xr[k].v[j]);
+            d[j] = to_f32(dr[k].v[j]);
+          }
+          win.push(v);
+          if (SILU) {
 #pragma unroll
-            for (int m = 0; m < W; ++m) u = __fmaf_rn(w[m][j], win.v[m][j], u);
-            const float g = sigmoid(u);
-            d[j] *= g * __fmaf_rn(u, 1.0f - g, 1.0f);
+            for (int j = 0; j < V; ++j) {
+              float u = bias[j];
+#pragma unroll
+              for (int m = 0; m < W; ++m) u = __fmaf_rn(w[m][j], win.v[m][j], u);
+              const float g = sigmoid(u);
+              d[j] *= g * __fmaf_rn(u, 1.0f - g, 1.0f);
+            }
+          }
+          if (t < to) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              db[j] += d[j];
+#pragma unroll
+              for (int m = 0; m < W; ++m) dw[m][j] = __fmaf_rn(d[j], win.v[m][j], dw[m][j]);
+            }
           }
         }
-        if (t < to) {
+        du.push(d);
+        const int64_t s = t - (W - 1);
+        float g[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            db[j] += d[j];
+        for (int j = 0; j < V; ++j) {
+          g[j] = 0.f;
 #pragma unroll
-            for (int m = 0; m < W; ++m) dw[m][j] = __fmaf_rn(d[j], win.v[m][j], dw[m][j]);
-          }
+          for (int m = 0; m < W; ++m) g[j] = __fmaf_rn(w[W - 1 - m][j], du.v[m][j], g[j]);
         }
-      }
-      du.push(d);
-      const int64_t s = t - (W - 1);
-      float g[V];
+        const int64_t fr = s - (end - (W - 1));  // its row in the final state
+        if (df && fr >= 0) {
+          float f[V];
+          load_pack<T, V>(df + (uint64_t)fr * a.channels, f);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        g[j] = 0.f;
-#pragma unroll
-        for (int m = 0; m < W; ++m) g[j] = __fmaf_rn(w[W - 1 - m][j], du.v[m][j], g[j]);
+          for (int j = 0; j < V; ++j) g[j] += f[j];
+        }
+        if (s >= from) store_pack<T, V>(dx + (uint64_t)s * a.dx_stride, g);
+        else if (ds && s < begin) store_pack<T, V>(ds + (uint64_t)(s - begin + W - 1) * a.channels, g);
       }
-      const int64_t fr = s - (end - (W - 1));  // its row in the final state
-      if (df && fr >= 0) {
-        float f[V];
-        load_pack<T, V>(df + (uint64_t)fr * a.channels, f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) g[j] += f[j];
-      }
-      if (s >= from) store_pack<T, V>(dx + (uint64_t)s * a.dx_stride, g);
-      else if (ds && s < begin) store_pack<T, V>(ds + (uint64_t)(s - begin + W - 1) * a.channels, g);
     }
     at = max(at, to);
   }
@@ -278,16 +316,22 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(ConvArgs a, uint32_
 
 enum Form { FORWARD, BACKWARD, STEP };
 
+// Channels of a block in the backward pass whatever the vectors: the tiles, and
+// so the workspace, must not depend on alignment.
+constexpr uint32_t kBackChannels = kThreads;
+
 template <Form F, class T, int V, int W, bool SILU>
 cudaError_t go(const ConvArgs& a, cudaStream_t s) {
   const uint32_t ctiles = (a.channels + kThreads * V - 1) / (kThreads * V);
-  const uint64_t tile = F == FORWARD ? kTile : F == BACKWARD ? kTileBack : 1;
+  const uint32_t tile = F == FORWARD    ? tile_of(a.seq.tokens, a.channels, kThreads * V)
+                        : F == BACKWARD ? tile_of(a.seq.tokens, a.channels, kBackChannels)
+                                        : 1;
   uint64_t tiles = (a.seq.tokens + tile - 1) / tile;
   if (tiles == 0) tiles = 1;  // sequences without tokens still have final states
   const uint64_t grid = tiles * ctiles;
   if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
-  if constexpr (F == FORWARD) conv_kernel<T, V, W, SILU><<<(unsigned)grid, kThreads, 0, s>>>(a, ctiles);
-  else if constexpr (F == BACKWARD) conv_backward_kernel<T, V, W, SILU><<<(unsigned)grid, kThreads, 0, s>>>(a, ctiles);
+  if constexpr (F == FORWARD) conv_kernel<T, V, W, SILU><<<(unsigned)grid, kThreads, 0, s>>>(a, ctiles, tile);
+  else if constexpr (F == BACKWARD) conv_backward_kernel<T, V, W, SILU><<<(unsigned)grid, kThreads, 0, s>>>(a, ctiles, tile);
   else conv_step_kernel<T, V, W, SILU><<<(unsigned)grid, kThreads, 0, s>>>(a, ctiles);
   return cudaGetLastError();
 }
@@ -358,9 +402,16 @@ cudaError_t launch_reduce_rows(const float* part, uint64_t rows, uint64_t cols, 
   return cudaGetLastError();
 }
 
+namespace {
+uint64_t back_tiles(uint64_t tokens, uint64_t channels) {
+  const uint32_t tile = tile_of(tokens, channels, kBackChannels);
+  const uint64_t tiles = (tokens + tile - 1) / tile;
+  return tiles ? tiles : 1;
+}
+}  // namespace
+
 size_t conv_backward_bytes(uint64_t tokens, uint64_t channels, uint32_t width) {
-  uint64_t tiles = (tokens + kTileBack - 1) / kTileBack;
-  return (tiles ? tiles : 1) * (width + 1) * channels * 4;
+  return back_tiles(tokens, channels) * (width + 1) * channels * 4;
 }
 
 cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s) { return by_type<FORWARD>(a, s); }
@@ -368,11 +419,9 @@ cudaError_t launch_conv_step(const ConvArgs& a, cudaStream_t s) { return by_type
 cudaError_t launch_conv_backward(const ConvArgs& a, cudaStream_t s) {
   cudaError_t e = by_type<BACKWARD>(a, s);
   if (e != cudaSuccess) return e;
-  uint64_t tiles = (a.seq.tokens + kTileBack - 1) / kTileBack;
-  if (tiles == 0) tiles = 1;
   // A partial row holds dw's channels * width sums, then dbias's.
   const uint64_t split = (uint64_t)a.channels * a.width;
-  return launch_reduce_rows(a.part, tiles, split + a.channels, split, a.dw, a.dbias, s);
+  return launch_reduce_rows(a.part, back_tiles(a.seq.tokens, a.channels), split + a.channels, split, a.dw, a.dbias, s);
 }
 
 }  // namespace sparsl

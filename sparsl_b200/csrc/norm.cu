@@ -16,12 +16,12 @@
 namespace sparsl {
 namespace {
 
-constexpr int kValues = 32;  // of a row, per thread, at most
 constexpr uint32_t kSms = 148;
 
-// Sums of v over the B threads that share a row.
+// Sums of v over the B threads that share a row; `turn` alternates from sum to
+// sum, so that one barrier does.
 template <int B, int M>
-__device__ __forceinline__ void row_sum(float (&v)[M], float* sh) {
+__device__ __forceinline__ void row_sum(float (&v)[M], float (*sh)[32 * M], int& turn) {
 #pragma unroll
   for (int o = 16; o; o >>= 1)
 #pragma unroll
@@ -29,73 +29,91 @@ __device__ __forceinline__ void row_sum(float (&v)[M], float* sh) {
   if constexpr (B > 32) {
     constexpr int kW = B / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    __syncthreads();  // the last sum's readers are done
+    float* s = sh[turn];
+    turn ^= 1;
     if (lane == 0)
 #pragma unroll
-      for (int m = 0; m < M; ++m) sh[warp * M + m] = v[m];
+      for (int m = 0; m < M; ++m) s[warp * M + m] = v[m];
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      float s = lane < kW ? sh[lane * M + m] : 0.f;
+      v[m] = lane < kW ? s[lane * M + m] : 0.f;
 #pragma unroll
-      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      v[m] = s;
+      for (int o = kW / 2; o; o >>= 1) v[m] += __shfl_xor_sync(0xffffffffu, v[m], o);
+      v[m] = __shfl_sync(0xffffffffu, v[m], 0);
     }
   }
 }
 
-// B threads per row (a block of at least 128), V values per access, I accesses
-// per thread.
+// B threads per row (several rows side by side in a block of 128 where B is
+// smaller), V values per access, I accesses per thread.  A block walks the rows
+// with weight and bias in registers, the next row asked for while one is done:
+// with a block per row the parameters' traffic from L2 was twice the rows'
+// (85 us against 34 at 16384 x 2048 bf16).
 template <class T, int V, int B, int I>
 __global__ void __launch_bounds__(B < 128 ? 128 : B) norm_kernel(NormArgs a) {
-  __shared__ float sh[32];
-  const uint32_t tid = B < 128 ? threadIdx.x % B : threadIdx.x;
-  const uint64_t row = B < 128 ? (uint64_t)blockIdx.x * (128 / B) + threadIdx.x / B : blockIdx.x;
-  if (row >= a.rows) return;
-  const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
-  float v[I][V];
-  float s[1] = {0.f};
+  __shared__ float sh[2][32];
+  constexpr int kSide = B < 128 ? 128 / B : 1;
+  const uint32_t tid = threadIdx.x % B;
+  const uint64_t step = (uint64_t)gridDim.x * kSide;
+  uint64_t row = (uint64_t)blockIdx.x * kSide + threadIdx.x / B;
+  float w[I][V], bias[I][V];
+  Pack<T, V> next[I];
+  const auto ask = [&](uint64_t r) {
+    const T* x = reinterpret_cast<const T*>(a.x) + r * a.x_stride;
 #pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const uint32_t c = (i * B + tid) * V;
-    if (c < a.channels) load_pack<T, V>(x + c, v[i]);
-    else
+    for (int i = 0; i < I; ++i) {
+      const uint32_t c = (i * B + tid) * V;
+      if (c < a.channels) next[i] = *reinterpret_cast<const Pack<T, V>*>(x + c);
+    }
+  };
+  if (row < a.rows) ask(row);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[0] += v[i][j];
-  }
-  row_sum<B>(s, sh);
-  const float mean = s[0] / (float)a.channels;
-  s[0] = 0.f;
-#pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const uint32_t c = (i * B + tid) * V;
+  for (int i = 0; i < I; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      v[i][j] -= mean;
-      if (c < a.channels) s[0] = __fmaf_rn(v[i][j], v[i][j], s[0]);
+      const uint32_t c = (i * B + tid) * V + j;
+      w[i][j] = a.w && c < a.channels ? load_param<T>(a.w, a.params_f32, c) : 1.f;
+      bias[i][j] = a.bias && c < a.channels ? load_param<T>(a.bias, a.params_f32, c) : 0.f;
     }
-  }
-  row_sum<B>(s, sh);
-  const float rstd = 1.0f / sqrtf(s[0] / (float)a.channels + a.eps);
-  if (tid == 0) {
-    if (a.mean) a.mean[row] = mean;
-    if (a.rstd) a.rstd[row] = rstd;
-  }
-  T* y = reinterpret_cast<T*>(a.y) + row * a.y_stride;
+  const float channels = (float)a.channels;
+  int turn = 0;
+  for (; row < a.rows; row += step) {
+    float v[I][V], s[1] = {0.f};
 #pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const uint32_t c = (i * B + tid) * V;
-    if (c >= a.channels) continue;
-    float o[V];
+    for (int i = 0; i < I; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      o[j] = v[i][j] * rstd;
-      if (a.w) o[j] = o[j] * load_param<T>(a.w, a.params_f32, c + j);
-      if (a.bias) o[j] += load_param<T>(a.bias, a.params_f32, c + j);
+      for (int j = 0; j < V; ++j) {
+        v[i][j] = (i * B + tid) * V < a.channels ? to_f32(next[i].v[j]) : 0.f;
+        s[0] += v[i][j];
+      }
+    if (row + step < a.rows) ask(row + step);
+    row_sum<B>(s, sh, turn);
+    const float mean = s[0] / channels;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[i][j] -= mean;
+        if ((i * B + tid) * V < a.channels) s[0] = __fmaf_rn(v[i][j], v[i][j], s[0]);
+      }
+    row_sum<B>(s, sh, turn);
+    const float rstd = 1.0f / sqrtf(s[0] / channels + a.eps);
+    if (tid == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
     }
-    store_pack<T, V>(y + c, o);
+    T* y = reinterpret_cast<T*>(a.y) + row * a.y_stride;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const uint32_t c = (i * B + tid) * V;
+      if (c >= a.channels) continue;
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = __fmaf_rn(v[i][j] * rstd, w[i][j], bias[i][j]);
+      store_pack<T, V>(y + c, o);
+    }
   }
 }
 
@@ -103,19 +121,20 @@ __global__ void __launch_bounds__(B < 128 ? 128 : B) norm_kernel(NormArgs a) {
 // second and third from the caches).
 template <class T>
 __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
-  __shared__ float sh[32];
+  __shared__ float sh[2][32];
+  int turn = 0;
   const uint64_t row = blockIdx.x;
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
   float s[1] = {0.f};
   for (uint64_t c = threadIdx.x; c < a.channels; c += 1024) s[0] += to_f32(x[c]);
-  row_sum<1024>(s, sh);
+  row_sum<1024>(s, sh, turn);
   const float mean = s[0] / (float)a.channels;
   s[0] = 0.f;
   for (uint64_t c = threadIdx.x; c < a.channels; c += 1024) {
     const float d = to_f32(x[c]) - mean;
     s[0] = __fmaf_rn(d, d, s[0]);
   }
-  row_sum<1024>(s, sh);
+  row_sum<1024>(s, sh, turn);
   const float rstd = 1.0f / sqrtf(s[0] / (float)a.channels + a.eps);
   if (threadIdx.x == 0) {
     if (a.mean) a.mean[row] = mean;
@@ -132,9 +151,26 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
 
 template <class T, int V, int B, int I>
 __global__ void __launch_bounds__(B) norm_backward_kernel(NormArgs a) {
-  __shared__ float sh[64];
+  __shared__ float sh[2][64];
   const uint32_t tid = threadIdx.x;
   float w[I][V], dw[I][V], db[I][V];
+  Pack<T, V> xn[I], dn[I];
+  float mean_n = 0.f, rstd_n = 0.f;
+  const auto ask = [&](uint64_t row) {
+    const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
+    const T* dy = reinterpret_cast<const T*>(a.dy) + row * a.dy_stride;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const uint32_t c = (i * B + tid) * V;
+      if (c < a.channels) {
+        xn[i] = *reinterpret_cast<const Pack<T, V>*>(x + c);
+        dn[i] = *reinterpret_cast<const Pack<T, V>*>(dy + c);
+      }
+    }
+    mean_n = a.mean[row];
+    rstd_n = a.rstd[row];
+  };
+  if (blockIdx.x < a.rows) ask(blockIdx.x);
 #pragma unroll
   for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -144,34 +180,25 @@ __global__ void __launch_bounds__(B) norm_backward_kernel(NormArgs a) {
       dw[i][j] = db[i][j] = 0.f;
     }
   const float scale = 1.0f / (float)a.channels;
+  int turn = 0;
   for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
-    const T* dy = reinterpret_cast<const T*>(a.dy) + row * a.dy_stride;
-    const float mean = a.mean[row], rstd = a.rstd[row];
+    const float mean = mean_n, rstd = rstd_n;
     float h[I][V], g[I][V], s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const uint32_t c = (i * B + tid) * V;
-      if (c < a.channels) {
-        load_pack<T, V>(x + c, h[i]);
-        load_pack<T, V>(dy + c, g[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) h[i][j] = mean, g[i][j] = 0.f;
-      }
-    }
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        h[i][j] = (h[i][j] - mean) * rstd;
+        const bool in = (i * B + tid) * V < a.channels;
+        h[i][j] = in ? (to_f32(xn[i].v[j]) - mean) * rstd : 0.f;
+        g[i][j] = in ? to_f32(dn[i].v[j]) : 0.f;
         db[i][j] += g[i][j];
         dw[i][j] = __fmaf_rn(g[i][j], h[i][j], dw[i][j]);
         g[i][j] *= w[i][j];
         s[0] += g[i][j];
         s[1] = __fmaf_rn(g[i][j], h[i][j], s[1]);
       }
-    row_sum<B>(s, sh);
+    if (row + gridDim.x < a.rows) ask(row + gridDim.x);
+    row_sum<B>(s, sh, turn);
     const float m0 = s[0] * scale, m1 = s[1] * scale;
     T* dx = reinterpret_cast<T*>(a.dx) + row * a.dx_stride;
 #pragma unroll
@@ -199,7 +226,8 @@ __global__ void __launch_bounds__(B) norm_backward_kernel(NormArgs a) {
 
 template <class T>
 __global__ void __launch_bounds__(1024) norm_long_dx_kernel(NormArgs a) {
-  __shared__ float sh[64];
+  __shared__ float sh[2][64];
+  int turn = 0;
   const uint64_t row = blockIdx.x;
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
   const T* dy = reinterpret_cast<const T*>(a.dy) + row * a.dy_stride;
@@ -210,7 +238,7 @@ __global__ void __launch_bounds__(1024) norm_long_dx_kernel(NormArgs a) {
     s[0] += g;
     s[1] = __fmaf_rn(g, (to_f32(x[c]) - mean) * rstd, s[1]);
   }
-  row_sum<1024>(s, sh);
+  row_sum<1024>(s, sh, turn);
   const float scale = 1.0f / (float)a.channels;
   T* dx = reinterpret_cast<T*>(a.dx) + row * a.dx_stride;
   for (uint64_t c = threadIdx.x; c < a.channels; c += 1024) {
@@ -237,37 +265,33 @@ __global__ void __launch_bounds__(256) norm_long_params_kernel(NormArgs a, uint3
   part[a.channels + c] = db;
 }
 
-constexpr uint64_t kLongBack = 8192;  // channels that 512 threads keep with their sums (16 values each)
+// Partial rows of dw and dbias: a block each.
 uint64_t back_parts(uint64_t rows) {
-  const uint64_t most = 2 * kSms;
+  const uint64_t most = 4 * kSms;
   return rows < most ? (rows ? rows : 1) : most;
 }
 
 template <class T, int V, int B, int I>
 cudaError_t go(const NormArgs& a, cudaStream_t s) {
-  const uint64_t grid = B < 128 ? (a.rows + 128 / B - 1) / (128 / B) : a.rows;
-  if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
-  norm_kernel<T, V, B, I><<<(unsigned)grid, B < 128 ? 128 : B, 0, s>>>(a);
+  constexpr uint64_t kSide = B < 128 ? 128 / B : 1;
+  const uint64_t blocks = (a.rows + kSide - 1) / kSide, most = (uint64_t)kSms * (B < 128 ? 12 : B >= 1024 ? 2 : 1536 / B);
+  norm_kernel<T, V, B, I><<<(unsigned)(blocks < most ? blocks : most), B < 128 ? 128 : B, 0, s>>>(a);
   return cudaGetLastError();
 }
 
+// 8 values of a row per thread, 16 where 1024 threads of 8 do not hold it: rows
+// up to 16384 values; longer ones are read again for each of the steps.
 template <class T, int V>
 cudaError_t forward(const NormArgs& a, cudaStream_t s) {
-  // Half as many values per thread where the rows are too few to fill the GPU.
-  constexpr int I = kValues / V, F = I >= 4 ? I / 4 : 1, H = I >= 2 ? I / 2 : 1;
+  constexpr int I = 8 / V;
   const uint64_t c = a.channels;
-  if (a.rows <= 2 * kSms) {
-    if (c <= 32 * F * V) return go<T, V, 32, F>(a, s);
-    if (c <= 128 * F * V) return go<T, V, 128, F>(a, s);
-    if (c <= 512 * F * V) return go<T, V, 512, F>(a, s);
-    if (c <= 1024 * F * V) return go<T, V, 1024, F>(a, s);
-  }
-  if (c <= 32 * H * V) return go<T, V, 32, H>(a, s);
-  if (c <= 128 * H * V) return go<T, V, 128, H>(a, s);
-  if (c <= 256 * H * V) return go<T, V, 256, H>(a, s);
-  if (c <= 512 * H * V) return go<T, V, 512, H>(a, s);
-  if (c <= 1024 * H * V) return go<T, V, 1024, H>(a, s);
-  if (c <= 1024 * I * V) return go<T, V, 1024, I>(a, s);
+  if (c <= 256) return go<T, V, 32, I>(a, s);
+  if (c <= 1024) return go<T, V, 128, I>(a, s);
+  if (c <= 2048) return go<T, V, 256, I>(a, s);
+  if (c <= 4096) return go<T, V, 512, I>(a, s);
+  if (c <= 6144) return go<T, V, 512, 12 / V + (12 % V ? 1 : 0)>(a, s);
+  if (c <= 8192) return go<T, V, 1024, I>(a, s);
+  if (c <= 16384) return go<T, V, 1024, 2 * I>(a, s);
   if (a.rows > 0x7fffffffull) return cudaErrorInvalidValue;
   norm_long_kernel<T><<<(unsigned)a.rows, 1024, 0, s>>>(a);
   return cudaGetLastError();
@@ -279,14 +303,18 @@ cudaError_t go_back(const NormArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+// 8 values per thread up to rows of 4096, 12 and 16 up to 6144 and 8192; longer
+// rows' dx and sums take a kernel each.
 template <class T, int V>
 cudaError_t backward(const NormArgs& a, cudaStream_t s) {
-  constexpr int H = kValues / 2 / V;  // 16 values per thread: x, dy and two sums of each
+  constexpr int I = 8 / V;
   const uint64_t c = a.channels;
-  if (c <= 64 * H * V) return go_back<T, V, 64, H>(a, s);
-  if (c <= 128 * H * V) return go_back<T, V, 128, H>(a, s);
-  if (c <= 256 * H * V) return go_back<T, V, 256, H>(a, s);
-  if (c <= 512 * H * V) return go_back<T, V, 512, H>(a, s);
+  if (c <= 512) return go_back<T, V, 64, I>(a, s);
+  if (c <= 1024) return go_back<T, V, 128, I>(a, s);
+  if (c <= 2048) return go_back<T, V, 256, I>(a, s);
+  if (c <= 4096) return go_back<T, V, 512, I>(a, s);
+  if (c <= 6144) return go_back<T, V, 512, 12 / V + (12 % V ? 1 : 0)>(a, s);
+  if (c <= 8192) return go_back<T, V, 512, 2 * I>(a, s);
   if (a.rows > 0x7fffffffull) return cudaErrorInvalidValue;
   norm_long_dx_kernel<T><<<(unsigned)a.rows, 1024, 0, s>>>(a);
   const uint64_t shares = back_parts(a.rows), blocks = (c + 255) / 256 * shares;

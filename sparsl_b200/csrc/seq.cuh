@@ -58,6 +58,21 @@ struct SeqView {
     }
     return lo;
   }
+  // The same by a whole warp: 32 probes at a time instead of one.
+  __device__ __forceinline__ int64_t first_from_warp(int64_t t) const {
+    if (!seq_ptr) return first_from(t);
+    const uint32_t lane = threadIdx.x & 31;
+    int64_t lo = 0, len = (int64_t)n_seq;  // the answer lies in [lo, lo + len]
+    while (len > 32) {
+      const int64_t each = (len + 31) / 32, at = lo + lane * each;
+      const uint32_t n = __popc(__ballot_sync(0xffffffffu, at < lo + len && begin(at) < t));
+      if (n == 0) return lo;
+      const int64_t end = lo + len;
+      lo += (n - 1) * each + 1;
+      len = lo + each - 1 < end ? each - 1 : end - lo;
+    }
+    return lo + __popc(__ballot_sync(0xffffffffu, lane < len && begin(lo + lane) < t));
+  }
   // The state row of sequence i, or -1.
   __device__ __forceinline__ int64_t slot(int64_t i) const {
     const int64_t s = slots ? (int64_t)__ldg(slots + i) : i;

@@ -40,6 +40,33 @@ struct OnDevice {
   }
 };
 
+// Whether [p, p + bytes) lies in one allocation of the GPU's own memory, by one
+// driver call; anything else is left to check_device_array, which says why.
+bool inside_allocation(const void* p, uint64_t bytes, int ordinal) {
+  typedef int (*GetAttributes)(unsigned int, int*, void**, unsigned long long);
+  static const GetAttributes get = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuPointerGetAttributes", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<GetAttributes>(f);
+  }();
+  if (!get) return false;
+  // CU_POINTER_ATTRIBUTE_{MEMORY_TYPE, DEVICE_ORDINAL, RANGE_START_ADDR, RANGE_SIZE, IS_MANAGED}
+  int which[5] = {2, 9, 11, 12, 8};
+  unsigned int type = 0;
+  int device = -1;
+  unsigned long long start = 0;
+  size_t size = 0;
+  unsigned char managed = 1;
+  void* out[5] = {&type, &device, &start, &size, &managed};
+  const unsigned long long at = reinterpret_cast<unsigned long long>(p);
+  if (get(5, which, out, at) != 0) return false;
+  return type == 2 /* CU_MEMORYTYPE_DEVICE */ && device == ordinal && !managed && at >= start && at - start <= size &&
+         bytes <= size - (at - start);
+}
+
 constexpr uint64_t kMostRows = 0x7fffffffull;  // seq_ptr's type
 constexpr uint64_t kMostBytes = 1ull << 62;
 
@@ -105,10 +132,12 @@ struct Call {
       fail(SPARSL_ERR_INVALID, "alignment", std::string(name) + ": not aligned to its elements");
       return;
     }
-    const int c = check_device_array(p, a.bytes(), ordinal, name);
-    if (c != SPARSL_OK) {
-      rc = c;
-      return;
+    if (!inside_allocation(p, a.bytes(), ordinal)) {
+      const int c = check_device_array(p, a.bytes(), ordinal, name);
+      if (c != SPARSL_OK) {
+        rc = c;
+        return;
+      }
     }
     arrays[count++] = a;
   }

@@ -325,27 +325,35 @@ template <class T, int LP>
 struct WarpRows {
   static constexpr int kCols = 32 / LP, kBytes = kCols * (int)sizeof(T), kPiece = kBytes < 16 ? kBytes : 16, kPieces = kBytes / kPiece;
   static constexpr int kLanes = kBatch * kPieces;  // pieces of one array's batch
+  template <int A, int PIECE>
+  static __device__ __forceinline__ void pieces(T (*to)[kBatch][kCols], const RowsIn (&from)[A], int64_t t, uint32_t live,
+                                                uint32_t c0, uint32_t cols) {
+    constexpr uint32_t kN = kBytes / PIECE;
+#pragma unroll
+    for (int it = 0; it < (int)(A * kBatch * kN + 31) / 32; ++it) {
+      const uint32_t i = it * 32 + (threadIdx.x & 31), piece = i % kN, k = i / kN % kBatch, which = i / (kN * kBatch);
+      if (which >= A || !(live >> k & 1)) continue;
+      RowsIn r = from[0];
+#pragma unroll
+      for (int q = 1; q < A; ++q)
+        if (which == (uint32_t)q) r = from[q];
+      const uint32_t first = piece * PIECE, have = cols * (uint32_t)sizeof(T);
+      if (have <= first) continue;
+      copy_async<PIECE>(reinterpret_cast<char*>(&to[which][k][0]) + first,
+                        reinterpret_cast<const char*>(cell<T>(r.p, t + k, r.row, c0)) + first,
+                        have - first < PIECE ? have - first : PIECE);
+    }
+  }
   // Rows t.. of the arrays, from channel c0 on, `cols` of them, those that
-  // `live` names; PER pieces of the A arrays' batches for each lane.
+  // `live` names.  `aligned`: 2 where whole pieces are, 1 where 4 bytes are.
   template <int A>
   static __device__ __forceinline__ void in(T (*to)[kBatch][kCols], const RowsIn (&from)[A], int64_t t, uint32_t live,
-                                            uint32_t c0, uint32_t cols, bool aligned) {
+                                            uint32_t c0, uint32_t cols, int aligned) {
     const uint32_t lane = threadIdx.x & 31;
-    if (aligned) {
-#pragma unroll
-      for (int it = 0; it < (A * kLanes + 31) / 32; ++it) {
-        const uint32_t i = it * 32 + lane, piece = i % kPieces, k = i / kPieces % kBatch, which = i / kLanes;
-        if (which >= A || !(live >> k & 1)) continue;
-        RowsIn r = from[0];
-#pragma unroll
-        for (int q = 1; q < A; ++q)
-          if (which == (uint32_t)q) r = from[q];
-        const uint32_t first = piece * kPiece, have = cols * (uint32_t)sizeof(T);
-        if (have <= first) continue;
-        copy_async<kPiece>(reinterpret_cast<char*>(&to[which][k][0]) + first,
-                           reinterpret_cast<const char*>(cell<T>(r.p, t + k, r.row, c0)) + first,
-                           have - first < kPiece ? have - first : kPiece);
-      }
+    if (aligned == 2) {
+      pieces<A, kPiece>(to, from, t, live, c0, cols);
+    } else if (aligned == 1) {
+      pieces<A, 4>(to, from, t, live, c0, cols);
     } else {
 #pragma unroll
       for (int q = 0; q < A; ++q)
@@ -358,9 +366,9 @@ struct WarpRows {
   }
   // The batch's results: rows t.. of one array.
   static __device__ __forceinline__ void out(const T (&from)[kBatch][kCols], void* to, uint32_t row, int64_t t, uint32_t live,
-                                             uint32_t c0, uint32_t cols, bool aligned) {
+                                             uint32_t c0, uint32_t cols, int aligned) {
     const uint32_t lane = threadIdx.x & 31;
-    if (aligned && cols == kCols) {
+    if (aligned == 2 && cols == kCols) {
       using Piece = Pack<T, kPiece / (int)sizeof(T)>;
 #pragma unroll
       for (int it = 0; it < (kLanes + 31) / 32; ++it) {
@@ -377,13 +385,14 @@ struct WarpRows {
     }
   }
 };
-// Whether the pieces of a warp's channels start on their own size in every row.
+// 2 where the pieces of a warp's channels start on their own size in every row,
+// 1 where they start on 4 bytes.
 template <class T, int LP>
-bool rows_aligned(const SscanArgs& a, std::initializer_list<RowsIn> rows) {
+int rows_aligned(const SscanArgs& a, std::initializer_list<RowsIn> rows) {
   uint64_t bits = (uint64_t)(a.groups > 1 ? a.channels / a.groups : 0) * sizeof(T);
   for (const RowsIn& r : rows)
     if (r.p) bits |= reinterpret_cast<uint64_t>(r.p) | (a.seq.tokens > 1 ? r.row : 0);
-  return bits % WarpRows<T, LP>::kPiece == 0;
+  return bits % WarpRows<T, LP>::kPiece == 0 ? 2 : bits % 4 == 0 ? 1 : 0;
 }
 
 }  // namespace sparsl

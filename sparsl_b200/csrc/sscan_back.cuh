@@ -209,7 +209,7 @@ struct BackShared {
 // with the states kept in registers, then backwards.  EDGES: a sequence begins
 // or ends inside the block.
 template <class T, int NS, int LP, bool FULL, bool GATE>
-__global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(SscanArgs a, ScanPlan p, BackWork w, bool aligned) {
+__global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(SscanArgs a, ScanPlan p, BackWork w, int aligned) {
   constexpr int NP = NS * LP, NH = NS / 2, K = kBlock, kOwn = K / LP, kEach = K * 2 * NP / kScanThreads;
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   BackShared<T, NS, LP>& sh = *reinterpret_cast<BackShared<T, NS, LP>*>(shared_bytes);
@@ -543,7 +543,7 @@ cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
   }
-  const bool aligned = rows_aligned<T, LP>(a, {{a.x, a.x_row}, {a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row},
+  const int aligned = rows_aligned<T, LP>(a, {{a.x, a.x_row}, {a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row},
                                               {a.dx, a.dx_row}, {a.ddt, a.ddt_row}, {a.dz, a.dz_row}});
   kernel<<<(unsigned)grid, kScanThreads, bytes, s>>>(a, p, w, aligned);
   const uint64_t cells = a.seq.tokens * a.groups * 2 * a.states;
