@@ -11,7 +11,7 @@ namespace sparsl {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kRowsAhead = 8;      // rows in flight per thread, asked for while the batch before is computed
+constexpr int kRowsAhead = 8;      // rows in flight per thread
 constexpr int kRowsAheadBack = 4;  // of x and of dy each
 constexpr uint32_t kSms = 148;
 
@@ -97,7 +97,7 @@ __device__ __forceinline__ void load_weights(const ConvArgs& a, uint32_t c, floa
 // final states, so that only one thread reads and writes a channel of a state
 // and the pool may be updated in place.
 template <class T, int V, int W, bool SILU>
-__global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs a, uint32_t ctiles, uint32_t tokens_a_tile) {
+__global__ void __launch_bounds__(kThreads, 6) conv_kernel(ConvArgs a, uint32_t ctiles, uint32_t tokens_a_tile) {
   const uint32_t ct = blockIdx.x % ctiles;
   const int64_t tile = blockIdx.x / ctiles;
   const int64_t tokens = (int64_t)a.seq.tokens, n = (int64_t)a.seq.n_seq;
@@ -123,34 +123,63 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs a, uint32_t cti
     int64_t to = min(end, t1);
     if (mine) to = min(end, max(t1, begin + (W - 1)));
     if (from < to) {
-      Pack<T, V> now[kRowsAhead], next[kRowsAhead];
-      const auto ask = [&](int64_t t) {
+      // Eight rows are always on their way: a row's place is asked for again as soon as it is read.
+      constexpr int R = kRowsAhead;
+      const T* px = x + (uint64_t)from * a.x_stride;
+      T* py = y + (uint64_t)from * a.y_stride;
+      Pack<T, V> rows[R];
 #pragma unroll
-        for (int k = 0; k < kRowsAhead; ++k)
-          if (t + k < to) next[k] = *reinterpret_cast<const Pack<T, V>*>(x + (uint64_t)(t + k) * a.x_stride);
-      };
-      ask(from);
+      for (int k = 0; k < R; ++k) {
+        if (from + k < to) rows[k] = *reinterpret_cast<const Pack<T, V>*>(px);
+        px += a.x_stride;
+      }
       Taps<T, V, W> win;
       load_taps<T, V, W>(a, i, begin, from, c, win);
-      for (int64_t t = from; t < to; t += kRowsAhead) {
+      const auto token = [&](const Pack<T, V>& r) {
+        float v[V], u[V];
 #pragma unroll
-        for (int k = 0; k < kRowsAhead; ++k) now[k] = next[k];
-        ask(t + kRowsAhead);
+        for (int j = 0; j < V; ++j) v[j] = to_f32(r.v[j]);
+        win.push(v);
+        if constexpr (V % 2 == 0) {
 #pragma unroll
-        for (int k = 0; k < kRowsAhead; ++k) {
-          if (t + k >= to) break;
-          float v[V], u[V];
+          for (int j = 0; j < V; j += 2) {
+            f32x2 s = pair(bias[j], bias[j + 1]);
 #pragma unroll
-          for (int j = 0; j < V; ++j) v[j] = to_f32(now[k].v[j]);
-          win.push(v);
+            for (int m = 0; m < W; ++m) s = fma2(pair(w[m][j], w[m][j + 1]), pair(win.v[m][j], win.v[m][j + 1]), s);
+            unpair(s, u[j], u[j + 1]);
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             u[j] = bias[j];
 #pragma unroll
             for (int m = 0; m < W; ++m) u[j] = __fmaf_rn(w[m][j], win.v[m][j], u[j]);
-            if (SILU) u[j] = u[j] * sigmoid(u[j]);
           }
-          store_pack<T, V>(y + (uint64_t)(t + k) * a.y_stride, u);
+        }
+        if (SILU)
+#pragma unroll
+          for (int j = 0; j < V; ++j) u[j] = u[j] * sigmoid(u[j]);
+        store_pack<T, V>(py, u);
+        py += a.y_stride;
+      };
+      int64_t t = from;
+      for (; t + 2 * R <= to; t += R) {
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const Pack<T, V> r = rows[k];
+          rows[k] = *reinterpret_cast<const Pack<T, V>*>(px);
+          px += a.x_stride;
+          token(r);
+        }
+      }
+      for (; t < to; t += R) {
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          if (t + k >= to) break;
+          const Pack<T, V> r = rows[k];
+          if (t + k + R < to) rows[k] = *reinterpret_cast<const Pack<T, V>*>(px);
+          px += a.x_stride;
+          token(r);
         }
       }
       at = to;
@@ -353,7 +382,7 @@ cudaError_t by_width(const ConvArgs& a, cudaStream_t s) {
 // channels otherwise.
 template <Form F, class T>
 cudaError_t by_vector(const ConvArgs& a, cudaStream_t s) {
-  constexpr int V = 8 / sizeof(T);
+  constexpr int V = 8 / sizeof(T);  // 16-byte vectors' weights and taps leave too few warps: 114 us against 77 at 16384 x 4096 bf16
   uint64_t m = a.channels | a.x_stride | a.y_stride | a.dy_stride | a.dx_stride;
   uint64_t p = 0;
   for (const void* q : {a.x, (const void*)a.y, a.state, (const void*)a.final_state, a.dy, (const void*)a.dx,

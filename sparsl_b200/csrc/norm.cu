@@ -117,6 +117,118 @@ __global__ void __launch_bounds__(B < 128 ? 128 : B) norm_kernel(NormArgs a) {
   }
 }
 
+// The rows a thread works on next, its own values of them.  Whole accesses of 16
+// bytes are copied into shared memory while a row is computed, STAGES rows ahead
+// (loads into registers are waited for at the first exchange between lanes); a
+// thread reads what it copied itself, so no barrier is needed.  Single values,
+// whose copies would be as many instructions again, wait in registers.
+template <class T, int V, int B, int I, int ARRAYS, int STAGES>
+struct RowsAhead {
+  static constexpr bool kAsync = V > 1;
+  static constexpr int kStages = kAsync ? STAGES : 1;
+  static constexpr int kBytes = kAsync ? STAGES * ARRAYS * I * (int)sizeof(Pack<T, V>) : 0;  // per thread
+  Pack<T, V>* sh;  // [stage][array][access][thread]
+  Pack<T, V> held[kAsync ? 1 : ARRAYS][kAsync ? 1 : I];
+  uint32_t threads, tid;
+  uint64_t channels;
+  __device__ __forceinline__ RowsAhead(void* p, uint32_t tid_, uint64_t channels_)
+      : sh(static_cast<Pack<T, V>*>(p) + threadIdx.x), threads(blockDim.x), tid(tid_), channels(channels_) {}
+  __device__ __forceinline__ Pack<T, V>* at(int stage, int array, int i) const {
+    return sh + ((stage * ARRAYS + array) * I + i) * threads;
+  }
+  __device__ __forceinline__ void ask(int stage, int array, const T* row) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const uint32_t c = (i * B + tid) * V;
+      if (c >= channels) continue;
+      if constexpr (kAsync) copy_async<V * (int)sizeof(T)>(at(stage, array, i), row + c, V * (uint32_t)sizeof(T));
+      else held[array][i] = *reinterpret_cast<const Pack<T, V>*>(row + c);
+    }
+  }
+  __device__ __forceinline__ Pack<T, V> get(int stage, int array, int i) const {
+    if constexpr (kAsync) return *at(stage, array, i);
+    else return held[array][i];
+  }
+};
+
+// Many rows: up to 64 values per thread, so that a row's two sums cost little
+// beside it, a warp per row where that holds one (no barrier then), and the
+// parameters, which 64 values' registers have no room for, in shared memory.
+template <class T, int V, int B, int I, int STAGES>
+__global__ void __launch_bounds__(256) norm_rows_kernel(NormArgs a) {
+  extern __shared__ __align__(16) float params[];  // weight, then bias, each padded to whole accesses; the rows ahead
+  __shared__ float sh[2][32];
+  constexpr int kSide = 256 / B;
+  const uint32_t tid = threadIdx.x % B, padded = (uint32_t)((a.channels + 3) / 4 * 4);
+  const uint64_t step = (uint64_t)gridDim.x * kSide;
+  uint64_t row = (uint64_t)blockIdx.x * kSide + threadIdx.x / B;
+  const T* x = reinterpret_cast<const T*>(a.x);
+  using Ahead = RowsAhead<T, V, B, I, 1, STAGES>;
+  Ahead ahead(params + 2 * padded, tid, a.channels);
+#pragma unroll
+  for (int k = 0; k < Ahead::kStages; ++k) {
+    if (row + k * step < a.rows) ahead.ask(k, 0, x + (row + k * step) * a.x_stride);
+    copies_issued();
+  }
+  for (uint32_t c = threadIdx.x; c < padded; c += 256) {
+    params[c] = a.w && c < a.channels ? load_param<T>(a.w, a.params_f32, c) : 1.f;
+    params[padded + c] = a.bias && c < a.channels ? load_param<T>(a.bias, a.params_f32, c) : 0.f;
+  }
+  __syncthreads();
+  const float channels = (float)a.channels;
+  int turn = 0, stage = 0;
+  for (; row < a.rows; row += step, stage = stage + 1 == Ahead::kStages ? 0 : stage + 1) {
+    copies_but<Ahead::kStages - 1>();
+    float v[I][V], s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const bool in = (i * B + tid) * V < a.channels;
+      Pack<T, V> r;
+      if (in) r = ahead.get(stage, 0, i);
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[i][j] = in ? to_f32(r.v[j]) : 0.f;
+        part += v[i][j];
+      }
+      s[0] += part;
+    }
+    const uint64_t far = row + Ahead::kStages * step;
+    if (far < a.rows) ahead.ask(stage, 0, x + far * a.x_stride);
+    copies_issued();
+    row_sum<B>(s, sh, turn);
+    const float mean = s[0] / channels;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const bool in = (i * B + tid) * V < a.channels;
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[i][j] -= mean;
+        part = __fmaf_rn(v[i][j], v[i][j], part);
+      }
+      if (in) s[0] += part;
+    }
+    row_sum<B>(s, sh, turn);
+    const float rstd = 1.0f / sqrtf(s[0] / channels + a.eps);
+    if (tid == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
+    T* y = reinterpret_cast<T*>(a.y) + row * a.y_stride;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const uint32_t c = (i * B + tid) * V;
+      if (c >= a.channels) continue;
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = __fmaf_rn(v[i][j] * rstd, params[c + j], params[padded + c + j]);
+      store_pack<T, V>(y + c, o);
+    }
+  }
+}
+
 // Rows longer than the registers hold: 1024 threads, x read three times (the
 // second and third from the caches).
 template <class T>
@@ -149,28 +261,28 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(NormArgs a) {
   }
 }
 
-template <class T, int V, int B, int I>
+template <class T, int V, int B, int I, int STAGES>
 __global__ void __launch_bounds__(B) norm_backward_kernel(NormArgs a) {
+  extern __shared__ __align__(16) float rows_ahead[];
   __shared__ float sh[2][64];
   const uint32_t tid = threadIdx.x;
-  float w[I][V], dw[I][V], db[I][V];
-  Pack<T, V> xn[I], dn[I];
-  float mean_n = 0.f, rstd_n = 0.f;
-  const auto ask = [&](uint64_t row) {
-    const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
-    const T* dy = reinterpret_cast<const T*>(a.dy) + row * a.dy_stride;
-#pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const uint32_t c = (i * B + tid) * V;
-      if (c < a.channels) {
-        xn[i] = *reinterpret_cast<const Pack<T, V>*>(x + c);
-        dn[i] = *reinterpret_cast<const Pack<T, V>*>(dy + c);
-      }
+  const T* x = reinterpret_cast<const T*>(a.x);
+  const T* dy = reinterpret_cast<const T*>(a.dy);
+  using Ahead = RowsAhead<T, V, B, I, 2, STAGES>;
+  Ahead ahead(rows_ahead, tid, a.channels);
+  const uint64_t step = gridDim.x;
+  const auto ask = [&](int stage, uint64_t row) {
+    if (row < a.rows) {
+      ahead.ask(stage, 0, x + row * a.x_stride);
+      ahead.ask(stage, 1, dy + row * a.dy_stride);
     }
-    mean_n = a.mean[row];
-    rstd_n = a.rstd[row];
+    copies_issued();
   };
-  if (blockIdx.x < a.rows) ask(blockIdx.x);
+#pragma unroll
+  for (int k = 0; k < Ahead::kStages; ++k) ask(k, blockIdx.x + k * step);
+  float mean_n = 0.f, rstd_n = 0.f;
+  if (blockIdx.x < a.rows) mean_n = a.mean[blockIdx.x], rstd_n = a.rstd[blockIdx.x];
+  float w[I][V], dw[I][V], db[I][V];
 #pragma unroll
   for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -180,24 +292,32 @@ __global__ void __launch_bounds__(B) norm_backward_kernel(NormArgs a) {
       dw[i][j] = db[i][j] = 0.f;
     }
   const float scale = 1.0f / (float)a.channels;
-  int turn = 0;
-  for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  int turn = 0, stage = 0;
+  for (uint64_t row = blockIdx.x; row < a.rows; row += step, stage = stage + 1 == Ahead::kStages ? 0 : stage + 1) {
     const float mean = mean_n, rstd = rstd_n;
+    if (row + step < a.rows) mean_n = a.mean[row + step], rstd_n = a.rstd[row + step];
+    copies_but<Ahead::kStages - 1>();
     float h[I][V], g[I][V], s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < I; ++i)
+    for (int i = 0; i < I; ++i) {
+      const bool in = (i * B + tid) * V < a.channels;
+      Pack<T, V> xr, dr;
+      if (in) {
+        xr = ahead.get(stage, 0, i);
+        dr = ahead.get(stage, 1, i);
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const bool in = (i * B + tid) * V < a.channels;
-        h[i][j] = in ? (to_f32(xn[i].v[j]) - mean) * rstd : 0.f;
-        g[i][j] = in ? to_f32(dn[i].v[j]) : 0.f;
+        h[i][j] = in ? (to_f32(xr.v[j]) - mean) * rstd : 0.f;
+        g[i][j] = in ? to_f32(dr.v[j]) : 0.f;
         db[i][j] += g[i][j];
         dw[i][j] = __fmaf_rn(g[i][j], h[i][j], dw[i][j]);
         g[i][j] *= w[i][j];
         s[0] += g[i][j];
         s[1] = __fmaf_rn(g[i][j], h[i][j], s[1]);
       }
-    if (row + gridDim.x < a.rows) ask(row + gridDim.x);
+    }
+    ask(stage, row + Ahead::kStages * step);
     row_sum<B>(s, sh, turn);
     const float m0 = s[0] * scale, m1 = s[1] * scale;
     T* dx = reinterpret_cast<T*>(a.dx) + row * a.dx_stride;
@@ -279,17 +399,45 @@ cudaError_t go(const NormArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-// 8 values of a row per thread, 16 where 1024 threads of 8 do not hold it: rows
-// up to 16384 values; longer ones are read again for each of the steps.
+template <class K>
+cudaError_t allow(K kernel, int bytes) {
+  return bytes > 40 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;
+}
+
+template <class T, int V, int B, int VALUES>
+cudaError_t go_rows(const NormArgs& a, cudaStream_t s) {
+  constexpr int kSide = 256 / B, kStages = 2;
+  const int bytes = (int)((a.channels + 3) / 4 * 4 * 8) + 256 * RowsAhead<T, V, B, VALUES / V, 1, kStages>::kBytes;
+  const auto kernel = norm_rows_kernel<T, V, B, VALUES / V, kStages>;
+  const cudaError_t e = allow(kernel, bytes);
+  if (e != cudaSuccess) return e;
+  const uint64_t blocks = (a.rows + kSide - 1) / kSide, fit = 220 * 1024 / bytes, regs = VALUES >= 64 ? 2 : VALUES >= 24 ? 3 : 5;
+  const uint64_t most = (uint64_t)kSms * (fit < regs ? (fit ? fit : 1) : regs);
+  kernel<<<(unsigned)(blocks < most ? blocks : most), 256, bytes, s>>>(a);
+  return cudaGetLastError();
+}
+
+// Many rows of up to 8192 values in 16-byte accesses: norm_rows_kernel, 16 to 64
+// values per thread (36 us against 50 at 16384 x 2048 bf16; single values are
+// better kept in registers, 45 us against 62 at 4099 x 5003 f32).  Otherwise 8 values per thread, 16 where 1024 threads of 8 do not hold a row;
+// rows over 16384 values are read again for each of the steps.
 template <class T, int V>
 cudaError_t forward(const NormArgs& a, cudaStream_t s) {
   constexpr int I = 8 / V;
   const uint64_t c = a.channels;
+  if (V > 1 && a.rows >= 16 * kSms) {
+    if (c <= 512) return go_rows<T, V, 32, 16>(a, s);
+    if (c <= 1024) return go_rows<T, V, 32, 32>(a, s);
+    if (c <= 2048) return go_rows<T, V, 32, 64>(a, s);
+    if (c <= 4096) return go_rows<T, V, 256, 16>(a, s);
+    if (c <= 6144) return go_rows<T, V, 256, 24>(a, s);
+    if (c <= 8192) return go_rows<T, V, 256, 32>(a, s);
+  }
   if (c <= 256) return go<T, V, 32, I>(a, s);
   if (c <= 1024) return go<T, V, 128, I>(a, s);
   if (c <= 2048) return go<T, V, 256, I>(a, s);
   if (c <= 4096) return go<T, V, 512, I>(a, s);
-  if (c <= 6144) return go<T, V, 512, 12 / V + (12 % V ? 1 : 0)>(a, s);
+  if (V == 1 && c <= 6144) return go<T, V, 512, 12 / V + (12 % V ? 1 : 0)>(a, s);
   if (c <= 8192) return go<T, V, 1024, I>(a, s);
   if (c <= 16384) return go<T, V, 1024, 2 * I>(a, s);
   if (a.rows > 0x7fffffffull) return cudaErrorInvalidValue;
@@ -299,20 +447,27 @@ cudaError_t forward(const NormArgs& a, cudaStream_t s) {
 
 template <class T, int V, int B, int I>
 cudaError_t go_back(const NormArgs& a, cudaStream_t s) {
-  norm_backward_kernel<T, V, B, I><<<(unsigned)back_parts(a.rows), B, 0, s>>>(a);
+  // Two rows ahead; one where that leaves an SM a single block.
+  constexpr int kThree = RowsAhead<T, V, B, I, 2, 3>::kBytes * B, kStages = kThree <= 72 * 1024 ? 3 : 2;
+  const int bytes = RowsAhead<T, V, B, I, 2, kStages>::kBytes * B;
+  const auto kernel = norm_backward_kernel<T, V, B, I, kStages>;
+  const cudaError_t e = allow(kernel, bytes);
+  if (e != cudaSuccess) return e;
+  kernel<<<(unsigned)back_parts(a.rows), B, bytes, s>>>(a);
   return cudaGetLastError();
 }
 
-// 8 values per thread up to rows of 4096, 12 and 16 up to 6144 and 8192; longer
-// rows' dx and sums take a kernel each.
+// 16 values per thread (8 in rows of up to 512, 12 in those of up to 6144): a
+// row's sums cost half of what they do with 8.  Longer rows' dx and sums take a
+// kernel each.
 template <class T, int V>
 cudaError_t backward(const NormArgs& a, cudaStream_t s) {
   constexpr int I = 8 / V;
   const uint64_t c = a.channels;
   if (c <= 512) return go_back<T, V, 64, I>(a, s);
-  if (c <= 1024) return go_back<T, V, 128, I>(a, s);
-  if (c <= 2048) return go_back<T, V, 256, I>(a, s);
-  if (c <= 4096) return go_back<T, V, 512, I>(a, s);
+  if (c <= 1024) return go_back<T, V, 64, 2 * I>(a, s);
+  if (c <= 2048) return go_back<T, V, 128, 2 * I>(a, s);
+  if (c <= 4096) return go_back<T, V, 256, 2 * I>(a, s);
   if (c <= 6144) return go_back<T, V, 512, 12 / V + (12 % V ? 1 : 0)>(a, s);
   if (c <= 8192) return go_back<T, V, 512, 2 * I>(a, s);
   if (a.rows > 0x7fffffffull) return cudaErrorInvalidValue;

@@ -120,6 +120,24 @@ __device__ __forceinline__ void store_pack(T* p, const float (&in)[V]) {
   *reinterpret_cast<Pack<T, V>*>(p) = k;
 }
 
+// Copies into shared memory that nothing waits for before copies_done() (or,
+// with the last N groups still under way, copies_but<N>()).
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from, uint32_t bytes) {
+  const uint32_t s = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(from), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(s), "l"(from), "n"(BYTES), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_done() {
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 // 2^v and 1/v by the special function unit (relative error below 2^-22 and

@@ -302,20 +302,6 @@ __device__ __forceinline__ uint32_t first_bits(int64_t n) { return n >= 32 ? ~0u
 // load behind them, since a warp has few scoreboards for both.
 constexpr int kBatch = 8;
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const void* from, uint32_t bytes) {
-  const uint32_t s = (uint32_t)__cvta_generic_to_shared(to);
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(from), "r"(bytes) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(s), "l"(from), "n"(BYTES), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copies_done() {
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncwarp();
-}
-
 struct RowsIn {
   const void* p;
   uint32_t row;  // bytes

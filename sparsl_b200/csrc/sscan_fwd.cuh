@@ -310,57 +310,98 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArg
   }
 }
 
-// One token of each sequence: LP lanes share a channel, 4 states each, so a
-// warp reads 512 contiguous bytes of states.  A block keeps its channels' rows
-// of A for TOKENS sequences, whose states are all asked for before the first is
-// used: with one sequence a block the launch of blocks and A's traffic from L2
-// took as long as the states' from HBM (77 us against 51 for 512 tokens x 4096
-// channels x 16 states).
-template <class T, int LP, int TOKENS, bool FULL>
+// One token of each sequence.  Few sequences: a channel's states over LP lanes, 4
+// each, to have blocks for all SMs.
+template <class T, int LP, bool FULL>
 __global__ void __launch_bounds__(kScanThreads) sscan_step_kernel(SscanArgs a, uint32_t ctiles) {
   const uint32_t N = a.states;
-  const int64_t i0 = (int64_t)(blockIdx.x / ctiles) * TOKENS;
+  const int64_t i = blockIdx.x / ctiles;
   const uint32_t c = (blockIdx.x % ctiles) * (kScanThreads / LP) + threadIdx.x / LP;
   const uint32_t n0 = threadIdx.x % LP * 4;
+  const int64_t slot = a.seq.slot(i);
+  if (slot < 0) return;  // the whole block's
   const bool valid = c < a.channels;
-  const uint32_t cc = valid ? c : a.channels - 1, g = cc / (a.channels / a.groups);
-  float h[TOKENS][4], a2[4], xv[TOKENS], s[TOKENS], zv[TOKENS];
-  float* st[TOKENS];
-#pragma unroll
-  for (int u = 0; u < TOKENS; ++u) {
-    const int64_t i = i0 + u, slot = i < (int64_t)a.seq.n_seq ? a.seq.slot(i) : -1;
-    st[u] = slot >= 0 ? a.final_state + ((uint64_t)slot * a.channels + cc) * N : nullptr;
-    if (!st[u]) continue;  // the whole block's
-    load_states<4, FULL>(st[u], n0, N, h[u]);
-    xv[u] = to_f32(*cell<T>(a.x, i, a.x_row, cc));
-    s[u] = to_f32(*cell<T>(a.dt, i, a.dt_row, cc));
-    zv[u] = a.z ? to_f32(*cell<T>(a.z, i, a.z_row, cc)) : 0.f;
-  }
+  const uint32_t cc = valid ? c : a.channels - 1;
+  float* st = a.final_state + ((uint64_t)slot * a.channels + cc) * N;
+  float h[4], a2[4];
+  load_states<4, FULL>(st, n0, N, h);
   load_states<4, FULL>(a.a + (uint64_t)cc * N, n0, N, a2);
-  const float bias = a.dt_bias ? a.dt_bias[cc] : 0.f, dskip = a.d ? a.d[cc] : 0.f;
+  const uint32_t g = cc / (a.channels / a.groups);
+  const T* b = reinterpret_cast<const T*>(a.b) + (uint64_t)i * a.b_stride + (uint64_t)g * a.b_group;
+  const T* cv = reinterpret_cast<const T*>(a.c) + (uint64_t)i * a.c_stride + (uint64_t)g * a.c_group;
+  const float xv = to_f32(*cell<T>(a.x, i, a.x_row, cc));
+  float s = to_f32(*cell<T>(a.dt, i, a.dt_row, cc));
+  const float zv = a.z ? to_f32(*cell<T>(a.z, i, a.z_row, cc)) : 0.f;
+  if (a.dt_bias) s += a.dt_bias[cc];
+  if (a.softplus) s = softplus(s);
+  float o = 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) a2[j] *= kLog2e;
+  for (int j = 0; j < 4; ++j) {
+    if (FULL || n0 + j < N) {
+      h[j] = __fmaf_rn(ex2(s * (a2[j] * kLog2e)), h[j], s * xv * to_f32(b[n0 + j]));
+      o = __fmaf_rn(to_f32(cv[n0 + j]), h[j], o);
+    }
+  }
+  o = sum_lanes<LP>(o);
+  if (a.d) o = __fmaf_rn(a.d[cc], xv, o);
+  if (a.z) o *= zv * sigmoid(zv);
+  if (!valid) return;
+  store_states<4, FULL>(st, n0, N, h);
+  if (n0 == 0) *cell<T>(a.y, i, a.y_row, c) = from_f32<T>(o);
+}
+
+// Many sequences: up to 16 states a lane, as in the scan, and a block's channels
+// for kStepTokens of them, whose states are all asked for before the first is
+// used.  A lane of 4 states took 200 instructions a token, for the step, the
+// gate and the addresses over again in each: 84 us against HBM's 44 for 512
+// tokens x 4096 channels x 16 states.
+constexpr int kStepTokens = 4;
+template <class T, int NS, int LP, bool FULL>
+__global__ void __launch_bounds__(kScanThreads, kResident) sscan_step_many_kernel(SscanArgs a, uint32_t per_group, uint32_t ctiles) {
+  constexpr int NP = NS * LP;
+  __shared__ __align__(16) float bc[kStepTokens][2][NP];
+  const uint32_t N = a.states;
+  const ScanLane<NS, LP> me(a.channels, a.groups, per_group, blockIdx.x % ctiles);
+  const int64_t i0 = (int64_t)(blockIdx.x / ctiles) * kStepTokens;
+  f32x2 h[kStepTokens][NS / 2], a2[NS / 2];
+  float xv[kStepTokens], s[kStepTokens], zv[kStepTokens];
+  int64_t at[kStepTokens];
 #pragma unroll
-  for (int u = 0; u < TOKENS; ++u) {
-    if (!st[u]) continue;
+  for (int u = 0; u < kStepTokens; ++u) {
+    const int64_t i = i0 + u, slot = i < (int64_t)a.seq.n_seq ? a.seq.slot(i) : -1;
+    at[u] = slot < 0 ? -1 : (int64_t)(((uint64_t)slot * a.channels + me.c) * N);
+    if (at[u] < 0) continue;  // the whole block's
+    load_pairs<NS, FULL>(a.final_state + at[u], me.n0, N, h[u]);
+    xv[u] = to_f32(*cell<T>(a.x, i, a.x_row, me.c));
+    s[u] = to_f32(*cell<T>(a.dt, i, a.dt_row, me.c));
+    zv[u] = a.z ? to_f32(*cell<T>(a.z, i, a.z_row, me.c)) : 0.f;
+  }
+  for (uint32_t q = threadIdx.x; q < kStepTokens * 2 * NP; q += kScanThreads) {
+    const uint32_t n = q % NP, which = q / NP & 1, u = q / (2 * NP);
     const int64_t i = i0 + u;
-    const T* b = reinterpret_cast<const T*>(a.b) + (uint64_t)i * a.b_stride + (uint64_t)g * a.b_group;
-    const T* cv = reinterpret_cast<const T*>(a.c) + (uint64_t)i * a.c_stride + (uint64_t)g * a.c_group;
+    float v = 0.f;
+    if (i < (int64_t)a.seq.n_seq && n < N)
+      v = to_f32(reinterpret_cast<const T*>(which ? a.c : a.b)[(uint64_t)i * (which ? a.c_stride : a.b_stride) +
+                                                              (uint64_t)me.group * (which ? a.c_group : a.b_group) + n]);
+    bc[u][which][n] = v;
+  }
+  load_pairs<NS, FULL>(a.a + (uint64_t)me.c * N, me.n0, N, a2, kLog2e);
+  const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f, dskip = a.d ? a.d[me.c] : 0.f;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kStepTokens; ++u) {
+    if (at[u] < 0) continue;
     float step = s[u] + bias;
     if (a.softplus) step = softplus(step);
-    float o = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (FULL || n0 + j < N) {
-        h[u][j] = __fmaf_rn(ex2(step * a2[j]), h[u][j], step * xv[u] * to_f32(b[n0 + j]));
-        o = __fmaf_rn(to_f32(cv[n0 + j]), h[u][j], o);
-      }
-    o = sum_lanes<LP>(o);
+    f32x2 e[NS / 2];
+    decay<NS>(step, a2, e);
+    advance<NS, FULL>(e, step * xv[u], &bc[u][0][me.n0], me.n0, N, h[u]);
+    float o = sum_lanes<LP>(dot<NS>(&bc[u][1][me.n0], h[u]));
     o = __fmaf_rn(dskip, xv[u], o);
     if (a.z) o *= zv[u] * sigmoid(zv[u]);
-    if (!valid) continue;
-    store_states<4, FULL>(st[u], n0, N, h[u]);
-    if (n0 == 0) *cell<T>(a.y, i, a.y_row, c) = from_f32<T>(o);
+    if (!me.valid) continue;
+    store_pairs<NS, FULL>(a.final_state + at[u], me.n0, N, h[u]);
+    if (me.first) *cell<T>(a.y, i0 + u, a.y_row, me.c) = from_f32<T>(o);
   }
 }
 
@@ -398,12 +439,23 @@ cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
 template <class T, int LP, bool FULL>
 cudaError_t go_step(const SscanArgs& a, cudaStream_t s) {
   const uint32_t per = kScanThreads / LP, ctiles = (a.channels + per - 1) / per;
-  // Four sequences a block once the blocks are 16 to an SM all the same.
-  const bool many = a.seq.n_seq * ctiles >= 64 * kSms;
-  const uint64_t grid = (many ? (a.seq.n_seq + 3) / 4 : a.seq.n_seq) * ctiles;
+  const uint64_t grid = a.seq.n_seq * ctiles;
   if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
-  if (many) sscan_step_kernel<T, LP, 4, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, ctiles);
-  else sscan_step_kernel<T, LP, 1, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, ctiles);
+  sscan_step_kernel<T, LP, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, ctiles);
+  return cudaGetLastError();
+}
+
+// Whether the many sequences' kernel fills the SMs with two waves of blocks.
+template <int LP>
+bool many(const SscanArgs& a, uint32_t& per_group, uint64_t& grid) {
+  const uint32_t cpg = a.channels / a.groups;
+  per_group = (cpg + kScanThreads / LP - 1) / (kScanThreads / LP);
+  grid = (a.seq.n_seq + kStepTokens - 1) / kStepTokens * per_group * a.groups;
+  return grid >= 2 * kResident * kSms && grid <= 0x7fffffffull;
+}
+template <class T, int NS, int LP, bool FULL>
+cudaError_t go_many(const SscanArgs& a, uint32_t per_group, uint64_t grid, cudaStream_t s) {
+  sscan_step_many_kernel<T, NS, LP, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, per_group, per_group * a.groups);
   return cudaGetLastError();
 }
 
@@ -437,6 +489,15 @@ template <class T>
 cudaError_t step_by_states(const SscanArgs& a, cudaStream_t s) {
   const uint32_t N = a.states;
   const bool al = aligned16(a.a) && aligned16(a.final_state);
+  uint32_t per;
+  uint64_t grid;
+  if (N <= 8 && many<1>(a, per, grid)) return N == 8 && al ? go_many<T, 8, 1, true>(a, per, grid, s) : go_many<T, 8, 1, false>(a, per, grid, s);
+  if (N > 8 && N <= 16 && many<1>(a, per, grid))
+    return N == 16 && al ? go_many<T, 16, 1, true>(a, per, grid, s) : go_many<T, 16, 1, false>(a, per, grid, s);
+  if (N > 16 && N <= 32 && many<2>(a, per, grid))
+    return N == 32 && al ? go_many<T, 16, 2, true>(a, per, grid, s) : go_many<T, 16, 2, false>(a, per, grid, s);
+  if (N > 32 && many<4>(a, per, grid))
+    return N == 64 && al ? go_many<T, 16, 4, true>(a, per, grid, s) : go_many<T, 16, 4, false>(a, per, grid, s);
   if (N == 16 && al) return go_step<T, 4, true>(a, s);
   if (N == 8 && al) return go_step<T, 2, true>(a, s);
   if (N == 32 && al) return go_step<T, 8, true>(a, s);
