@@ -97,13 +97,14 @@ __device__ __forceinline__ void load_weights(const ConvArgs& a, uint32_t c, floa
 // final states, so that only one thread reads and writes a channel of a state
 // and the pool may be updated in place.
 template <class T, int V, int W, bool SILU>
-__global__ void __launch_bounds__(kThreads, 6) conv_kernel(ConvArgs a, uint32_t ctiles, uint32_t tokens_a_tile) {
+__global__ void __launch_bounds__(kThreads) conv_kernel(ConvArgs a, uint32_t ctiles, uint32_t tokens_a_tile) {
   const uint32_t ct = blockIdx.x % ctiles;
   const int64_t tile = blockIdx.x / ctiles;
   const int64_t tokens = (int64_t)a.seq.tokens, n = (int64_t)a.seq.n_seq;
   const int64_t t0 = tile * tokens_a_tile;
   const bool last = t0 + tokens_a_tile >= tokens;
   const int64_t t1 = last ? tokens : t0 + tokens_a_tile;
+  __shared__ __align__(16) Pack<T, V> ring[kRowsAhead][kThreads];
   int64_t i = a.seq.first_from_warp(t0);
   const uint32_t c = (ct * kThreads + threadIdx.x) * V;
   if (c >= a.channels) return;
@@ -123,16 +124,22 @@ __global__ void __launch_bounds__(kThreads, 6) conv_kernel(ConvArgs a, uint32_t 
     int64_t to = min(end, t1);
     if (mine) to = min(end, max(t1, begin + (W - 1)));
     if (from < to) {
-      // Eight rows are always on their way: a row's place is asked for again as soon as it is read.
+      // Eight rows are always on their way into shared memory, each thread's own
+      // columns of them (in registers, eight rows' loads and as many warps do not
+      // fit); two-byte columns, which cannot be copied, are loaded when wanted.
       constexpr int R = kRowsAhead;
+      constexpr bool kRing = V * sizeof(T) >= 4;
       const T* px = x + (uint64_t)from * a.x_stride;
       T* py = y + (uint64_t)from * a.y_stride;
-      Pack<T, V> rows[R];
+      const auto ask = [&](int slot, bool any) {
+        if constexpr (kRing) {
+          if (any) copy_async<V * (int)sizeof(T)>(&ring[slot][threadIdx.x], px, V * (uint32_t)sizeof(T));
+          px += a.x_stride;
+          copies_issued();
+        }
+      };
 #pragma unroll
-      for (int k = 0; k < R; ++k) {
-        if (from + k < to) rows[k] = *reinterpret_cast<const Pack<T, V>*>(px);
-        px += a.x_stride;
-      }
+      for (int k = 0; k < R; ++k) ask(k, from + k < to);
       Taps<T, V, W> win;
       load_taps<T, V, W>(a, i, begin, from, c, win);
       const auto token = [&](const Pack<T, V>& r) {
@@ -162,24 +169,30 @@ __global__ void __launch_bounds__(kThreads, 6) conv_kernel(ConvArgs a, uint32_t 
         store_pack<T, V>(py, u);
         py += a.y_stride;
       };
+      const auto take = [&](int k) {
+        if constexpr (kRing) {
+          copies_but<R - 1>();
+          return ring[k][threadIdx.x];
+        } else {
+          const Pack<T, V> r = *reinterpret_cast<const Pack<T, V>*>(px);
+          px += a.x_stride;
+          return r;
+        }
+      };
       int64_t t = from;
       for (; t + 2 * R <= to; t += R) {
 #pragma unroll
         for (int k = 0; k < R; ++k) {
-          const Pack<T, V> r = rows[k];
-          rows[k] = *reinterpret_cast<const Pack<T, V>*>(px);
-          px += a.x_stride;
-          token(r);
+          token(take(k));
+          ask(k, true);
         }
       }
       for (; t < to; t += R) {
 #pragma unroll
         for (int k = 0; k < R; ++k) {
           if (t + k >= to) break;
-          const Pack<T, V> r = rows[k];
-          if (t + k + R < to) rows[k] = *reinterpret_cast<const Pack<T, V>*>(px);
-          px += a.x_stride;
-          token(r);
+          token(take(k));
+          ask(k, t + k + R < to);
         }
       }
       at = to;
@@ -382,7 +395,7 @@ cudaError_t by_width(const ConvArgs& a, cudaStream_t s) {
 // channels otherwise.
 template <Form F, class T>
 cudaError_t by_vector(const ConvArgs& a, cudaStream_t s) {
-  constexpr int V = 8 / sizeof(T);  // 16-byte vectors' weights and taps leave too few warps: 114 us against 77 at 16384 x 4096 bf16
+  constexpr int V = 8 / sizeof(T);  // 16-byte vectors' weights and taps leave too few warps: 79 us against 55 at 16384 x 4096 bf16
   uint64_t m = a.channels | a.x_stride | a.y_stride | a.dy_stride | a.dx_stride;
   uint64_t p = 0;
   for (const void* q : {a.x, (const void*)a.y, a.state, (const void*)a.final_state, a.dy, (const void*)a.dx,

@@ -11,11 +11,13 @@ Outputs are the caller's arrays; an output must not overlap an input.
 """
 from __future__ import annotations
 
-from ctypes import byref
+import struct
 
 from . import _lib
 
 _CODES = {}  # dtype -> sparsl dtype code, for those seen
+_KINDS = {0: "float32", 1: "float16", 2: "bfloat16", 10: "int32", 11: "uint8"}
+_NONE = (0, 0)  # no rows
 
 
 def _code(t, name: str) -> int:
@@ -30,12 +32,11 @@ def _code(t, name: str) -> int:
     return c
 
 
-def _want(t, name: str, code: int, kind: str):
-    if _code(t, name) != code:
-        raise TypeError(f"`{name}` must be {kind}, got {t.dtype}")
-
-
-_KINDS = {0: "float32", 1: "float16", 2: "bfloat16", 10: "int32", 11: "uint8"}
+def _token_code(x) -> int:
+    c = _code(x, "x")
+    if c > 2:
+        raise TypeError("`x` must be float32, float16 or bfloat16")
+    return c
 
 
 def _length(what: str, got, expected):
@@ -45,95 +46,92 @@ def _length(what: str, got, expected):
                    expected=tuple(expected), got=tuple(got))
 
 
-def _fill_rows(to, t, name: str, shape, code: int):
-    """A token array into a ``sparsl_rows``."""
-    if tuple(t.shape) != shape:
+def _rows(t, name: str, shape, dtype):
+    """A token array as (address, row stride in elements)."""
+    if t.shape != shape:
         raise _length(name, t.shape, shape)
-    _want(t, name, code, _KINDS[code])
+    if t.dtype != dtype:
+        raise TypeError(f"`{name}` must be {dtype}, got {t.dtype}")
     st = t.stride()
     if st[1] != 1 and shape[1] > 1:
         raise TypeError(f"`{name}` must have its channels next to each other")
-    to.p = t.data_ptr()
-    to.stride = st[0] if shape[0] > 1 else shape[1]
+    return t.data_ptr(), st[0] if shape[0] > 1 else shape[1]
 
 
-def _fill_runs(to, t, name: str, tokens: int, groups: int, states: int, code: int) -> int:
-    """A [tokens, states] or [tokens, groups, states] array; returns the group stride."""
-    shape = tuple(t.shape)
+def _runs(t, name: str, tokens: int, groups: int, states: int, dtype):
+    """A [tokens, states] or [tokens, groups, states] array as (address, row stride, group stride)."""
+    shape = t.shape
     if shape != (tokens, groups, states) and not (groups == 1 and shape == (tokens, states)):
         raise _length(name, shape, (tokens, groups, states))
-    _want(t, name, code, _KINDS[code])
+    if t.dtype != dtype:
+        raise TypeError(f"`{name}` must be {dtype}, got {t.dtype}")
     st = t.stride()
     if st[-1] != 1 and states > 1:
         raise TypeError(f"`{name}` must have its states next to each other")
     group = st[1] if len(shape) == 3 and groups > 1 else states
-    to.p = t.data_ptr()
-    to.stride = st[0] if tokens > 1 else (groups - 1) * group + states
-    return group
+    return t.data_ptr(), st[0] if tokens > 1 else (groups - 1) * group + states, group
 
 
-def _flat(t, name: str, shape, code: int):
-    """The address of a contiguous array."""
-    if tuple(t.shape) != shape:
+def _flat(t, name: str, shape, code: int) -> int:
+    """The address of a contiguous array; 0 for None."""
+    if t is None:
+        return 0
+    if t.shape != shape:
         raise _length(name, t.shape, shape)
-    _want(t, name, code, _KINDS[code])
+    if _code(t, name) != code:
+        raise TypeError(f"`{name}` must be {_KINDS[code]}, got {t.dtype}")
     if not t.is_contiguous():
         raise TypeError(f"`{name}` must be contiguous")
     return t.data_ptr()
 
 
-def _params(named, shapes, token_code: int) -> int:
-    """Parameters are float32 or of the tokens' type, all alike: 1 for float32."""
-    f32 = None
-    for (name, t), shape in zip(named, shapes):
+def _params(weight, bias, token_code: int) -> int:
+    """Parameters are float32 or of the tokens' type, alike: the dtype code of both."""
+    code = None
+    for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
         c = _code(t, name)
-        if c not in (0, token_code) or (f32 is not None and f32 != (c == 0)):
+        if c not in (0, token_code) or (code is not None and c != code):
             raise TypeError(f"`{name}` must be float32 or have the tokens' dtype, like the other parameters")
-        f32 = c == 0
-    return 1 if f32 or f32 is None else 0
+        code = c
+    return 0 if code is None else code
 
 
-def _fill_seqs(s, tokens: int, seq_ptr, n_seq, slots=None, resume=None):
-    s.tokens = tokens
+def _seqs(tokens: int, seq_ptr, n_seq, slots, resume, n_slots: int):
+    """The fields of ``sparsl_seqs``."""
+    ptr = 0
     if seq_ptr is not None:
         n = seq_ptr.shape[0] - 1
         if n < 0 or (n_seq is not None and n_seq != n):
             raise _length("seq_ptr", seq_ptr.shape, ((n_seq if n_seq is not None else 0) + 1,))
-        s.seq_ptr = _flat(seq_ptr, "seq_ptr", (n + 1,), 10)
+        ptr = _flat(seq_ptr, "seq_ptr", (n + 1,), 10)
     else:
         n = 1 if n_seq is None else int(n_seq)
         if n < 0:
             raise ValueError("`n_seq` must not be negative")
-    s.n_seq = n
-    if slots is not None:
-        s.slots = _flat(slots, "slots", (n,), 10)
-    if resume is not None:
-        s.resume = _flat(resume, "resume", (n,), 11)
-    return n
+    return (tokens, n, ptr, _flat(slots, "slots", (n,), 10), _flat(resume, "resume", (n,), 11), n_slots)
 
 
-def _fill_states(s, arrays, tail, code: int):
-    """State arrays [rows, *tail], all with as many rows; their addresses by name."""
+def _states(arrays, tail, code: int):
+    """State arrays [rows, *tail], all with as many rows: (rows, their addresses)."""
     out, rows = [], None
     for name, t in arrays:
         if t is None:
-            out.append(None)
+            out.append(0)
             continue
         n = t.shape[0] if len(t.shape) else 0
         if rows is not None and n != rows:
             raise _length(name, t.shape, (rows, *tail))
         rows = n
         out.append(_flat(t, name, (n, *tail), code))
-    s.n_slots = rows or 0
-    return out
+    return rows or 0, out
 
 
 def _scratch(t):
     """(address, bytes) of a workspace."""
     if t is None:
-        return None, 0
+        return _NONE
     if hasattr(t, "is_contiguous") and not t.is_contiguous():
         raise TypeError("a workspace must be contiguous")
     return t.data_ptr(), t.numel() * t.element_size()
@@ -147,34 +145,35 @@ def _stream(stream):
     return stream.cuda_stream or 1  # cudaStreamLegacy
 
 
+# The argument blocks of include/sparsl_cuda.h, packed in one go (filling
+# ctypes structures field by field took longer than the launch).
+_CONV = struct.Struct("=6Q3i2I4x4Q4Q4Q2Q2Q2Q")
+_SCAN = struct.Struct("=6Q2i4I12Q2Q7Q12Q2Q5Q2Q")
+_NORM = struct.Struct("=2Q2i4Q4QfI4Q2Q2Q")
+
+
 class SequenceOps:
     """Mixed into ``Device``."""
 
-    def _run_sequence(self, fn: str, args, operation: str, stream):
-        rc = getattr(_lib.load(), fn)(self._h, byref(args), _stream(stream))
+    def _run_sequence(self, fn: str, args: bytes, operation: str, stream):
+        rc = getattr(_lib.load(), fn)(self._h, args, _stream(stream))
         if rc:
             from .backend import _check
 
             _check(rc, operation)
 
     # ---- the short causal convolution ----
-    def _conv_args(self, x, weight, bias, silu):
+    @staticmethod
+    def _conv_head(x, weight, bias, silu):
         tokens, channels = x.shape
         if len(weight.shape) != 2 or weight.shape[0] != channels:
             raise _length("weight", weight.shape, (channels, "width"))
         width = weight.shape[1]
-        a = _lib.ConvArgs()
-        code = _code(x, "x")
-        if code > 2:
-            raise TypeError("`x` must be float32, float16 or bfloat16")
-        a.dtype, a.silu, a.channels, a.width = code, int(bool(silu)), channels, width
-        a.params_f32 = _params((("weight", weight), ("bias", bias)), ((channels, width), (channels,)), code)
-        _fill_rows(a.x, x, "x", (tokens, channels), code)
-        pc = 0 if a.params_f32 else code
-        a.weight = _flat(weight, "weight", (channels, width), pc)
-        if bias is not None:
-            a.bias = _flat(bias, "bias", (channels,), pc)
-        return a, tokens, channels, width, code
+        code = _token_code(x)
+        pc = _params(weight, bias, code)
+        head = (code, 1 if pc == 0 else 0, 1 if silu else 0, channels, width)
+        params = (_flat(weight, "weight", (channels, width), pc), _flat(bias, "bias", (channels,), pc))
+        return tokens, channels, width, code, head, _rows(x, "x", (tokens, channels), x.dtype), params
 
     def causal_conv_device(self, x, weight, y, *, bias=None, silu: bool = False, seq_ptr=None, n_seq=None, state=None,
                            final_state=None, slots=None, resume=None, stream=None) -> None:
@@ -189,12 +188,12 @@ class SequenceOps:
         token; sequence i uses row ``slots[i]`` (int32; a negative one: none)
         or row i, starting from zero without ``state`` or where ``resume[i]``
         is 0.  ``final_state`` may be ``state`` itself."""
-        a, tokens, channels, width, code = self._conv_args(x, weight, bias, silu)
-        _fill_rows(a.y, y, "y", (tokens, channels), code)
-        _fill_seqs(a.seqs, tokens, seq_ptr, n_seq, slots, resume)
-        a.state, a.final_state = _fill_states(a.seqs, (("state", state), ("final_state", final_state)),
-                                              (width - 1, channels), code)
-        self._run_sequence("sparsl_dev_causal_conv_device", a, "causal_conv", stream)
+        tokens, channels, width, code, head, xr, params = self._conv_head(x, weight, bias, silu)
+        yr = _rows(y, "y", (tokens, channels), x.dtype)
+        rows, (st, fin) = _states((("state", state), ("final_state", final_state)), (width - 1, channels), code)
+        args = _CONV.pack(*_seqs(tokens, seq_ptr, n_seq, slots, resume, rows), *head, *xr, *yr, *params, st, fin,
+                          0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        self._run_sequence("sparsl_dev_causal_conv_device", args, "causal_conv", stream)
 
     @staticmethod
     def causal_conv_backward_workspace(tokens: int, channels: int, width: int) -> int:
@@ -209,54 +208,45 @@ class SequenceOps:
         overwritten.  Row i of the state arrays is sequence i's; ``dstate``
         receives the gradient of ``state``, ``dfinal_state`` holds that of the
         final state."""
-        a, tokens, channels, width, code = self._conv_args(x, weight, bias, silu)
-        _fill_rows(a.dy, dy, "dy", (tokens, channels), code)
-        _fill_rows(a.dx, dx, "dx", (tokens, channels), code)
-        a.dweight = _flat(dweight, "dweight", (channels, width), 0)
-        if dbias is not None:
-            a.dbias = _flat(dbias, "dbias", (channels,), 0)
-        _fill_seqs(a.seqs, tokens, seq_ptr, n_seq)
-        a.state, a.dstate, a.dfinal_state = _fill_states(
-            a.seqs, (("state", state), ("dstate", dstate), ("dfinal_state", dfinal_state)), (width - 1, channels), code)
-        a.workspace, a.workspace_bytes = _scratch(workspace)
-        self._run_sequence("sparsl_dev_causal_conv_backward_device", a, "causal_conv_backward", stream)
+        tokens, channels, width, code, head, xr, params = self._conv_head(x, weight, bias, silu)
+        shape = (tokens, channels)
+        dyr, dxr = _rows(dy, "dy", shape, x.dtype), _rows(dx, "dx", shape, x.dtype)
+        rows, (st, ds, df) = _states((("state", state), ("dstate", dstate), ("dfinal_state", dfinal_state)),
+                                     (width - 1, channels), code)
+        args = _CONV.pack(*_seqs(tokens, seq_ptr, n_seq, None, None, rows), *head, *xr, 0, 0, *params, st, 0, *dyr, *dxr,
+                          _flat(dweight, "dweight", (channels, width), 0), _flat(dbias, "dbias", (channels,), 0), ds, df,
+                          *_scratch(workspace))
+        self._run_sequence("sparsl_dev_causal_conv_backward_device", args, "causal_conv_backward", stream)
 
     def causal_conv_step_device(self, x, weight, y, state, *, bias=None, silu: bool = False, slots=None,
                                 stream=None) -> None:
         """One token of each sequence: ``x``, ``y`` [sequences, channels]; ``state``
         [rows, width - 1, channels] is updated in place.  Where ``slots[i]`` is
         negative, row i of y stays as it was."""
-        a, tokens, channels, width, code = self._conv_args(x, weight, bias, silu)
-        _fill_rows(a.y, y, "y", (tokens, channels), code)
-        _fill_seqs(a.seqs, tokens, None, tokens, slots)
-        (a.final_state,) = _fill_states(a.seqs, (("state", state),), (width - 1, channels), code)
-        self._run_sequence("sparsl_dev_causal_conv_step_device", a, "causal_conv_step", stream)
+        tokens, channels, width, code, head, xr, params = self._conv_head(x, weight, bias, silu)
+        yr = _rows(y, "y", (tokens, channels), x.dtype)
+        rows, (st,) = _states((("state", state),), (width - 1, channels), code)
+        args = _CONV.pack(*_seqs(tokens, None, tokens, slots, None, rows), *head, *xr, *yr, *params, 0, st,
+                          0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        self._run_sequence("sparsl_dev_causal_conv_step_device", args, "causal_conv_step", stream)
 
     # ---- the selective scan ----
-    def _scan_args(self, x, dt, a, b, c, d, z, dt_bias, softplus):
+    @staticmethod
+    def _scan_head(x, dt, a, b, c, d, z, dt_bias, softplus):
         tokens, channels = x.shape
         if len(a.shape) != 2 or a.shape[0] != channels:
             raise _length("a", a.shape, (channels, "states"))
         states = a.shape[1]
         groups = b.shape[1] if len(b.shape) == 3 else 1
-        code = _code(x, "x")
-        if code > 2:
-            raise TypeError("`x` must be float32, float16 or bfloat16")
-        k = _lib.ScanArgs()
-        k.dtype, k.softplus, k.channels, k.states, k.groups = code, int(bool(softplus)), channels, states, groups
-        shape = (tokens, channels)
-        _fill_rows(k.x, x, "x", shape, code)
-        _fill_rows(k.dt, dt, "dt", shape, code)
-        if z is not None:
-            _fill_rows(k.z, z, "z", shape, code)
-        k.b_group = _fill_runs(k.b, b, "b", tokens, groups, states, code)
-        k.c_group = _fill_runs(k.c, c, "c", tokens, groups, states, code)
-        k.a = _flat(a, "a", (channels, states), 0)
-        if d is not None:
-            k.d = _flat(d, "d", (channels,), 0)
-        if dt_bias is not None:
-            k.dt_bias = _flat(dt_bias, "dt_bias", (channels,), 0)
-        return k, tokens, channels, states, groups, code
+        code = _token_code(x)
+        kind, shape = x.dtype, (tokens, channels)
+        br, cr = _runs(b, "b", tokens, groups, states, kind), _runs(c, "c", tokens, groups, states, kind)
+        sizes = (code, 1 if softplus else 0, channels, states, groups, 0)
+        rows = (*_rows(x, "x", shape, kind), *_rows(dt, "dt", shape, kind),
+                *(_NONE if z is None else _rows(z, "z", shape, kind)), br[0], br[1], cr[0], cr[1])
+        params = (br[2], cr[2], _flat(a, "a", (channels, states), 0), _flat(d, "d", (channels,), 0),
+                  _flat(dt_bias, "dt_bias", (channels,), 0))
+        return tokens, channels, states, groups, sizes, rows, params
 
     @staticmethod
     def selective_scan_workspace(tokens: int, channels: int, states: int, n_seq: int = 1, groups: int = 1) -> int:
@@ -287,15 +277,12 @@ class SequenceOps:
         resume as in :meth:`causal_conv_device`; ``state`` / ``final_state``:
         [rows, channels, states] float32.  ``checkpoints`` keeps what
         :meth:`selective_scan_backward_device` needs."""
-        k, tokens, channels, states, groups, code = self._scan_args(x, dt, a, b, c, d, z, dt_bias, softplus)
-        _fill_rows(k.y, y, "y", (tokens, channels), code)
-        _fill_seqs(k.seqs, tokens, seq_ptr, n_seq, slots, resume)
-        k.state, k.final_state = _fill_states(k.seqs, (("state", state), ("final_state", final_state)),
-                                              (channels, states), 0)
-        if checkpoints is not None:
-            k.checkpoints, k.checkpoint_bytes = _scratch(checkpoints)
-        k.workspace, k.workspace_bytes = _scratch(workspace)
-        self._run_sequence("sparsl_dev_selective_scan_device", k, "selective_scan", stream)
+        tokens, channels, states, groups, sizes, rows, params = self._scan_head(x, dt, a, b, c, d, z, dt_bias, softplus)
+        n, (st, fin) = _states((("state", state), ("final_state", final_state)), (channels, states), 0)
+        args = _SCAN.pack(*_seqs(tokens, seq_ptr, n_seq, slots, resume, n), *sizes, *rows,
+                          *_rows(y, "y", (tokens, channels), x.dtype), *params, st, fin, *_scratch(checkpoints),
+                          0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, *_scratch(workspace))
+        self._run_sequence("sparsl_dev_selective_scan_device", args, "selective_scan", stream)
 
     def selective_scan_backward_device(self, dy, x, dt, a, b, c, checkpoints, dx, ddt, da, db, dc, workspace, *, d=None,
                                        dd=None, z=None, dz=None, dt_bias=None, ddt_bias=None, softplus: bool = False,
@@ -307,70 +294,47 @@ class SequenceOps:
         overwritten.  ``dz`` goes with ``z``.  Row i of the state arrays is
         sequence i's; ``dstate`` receives the gradient of ``state``,
         ``dfinal_state`` holds that of the final state."""
-        k, tokens, channels, states, groups, code = self._scan_args(x, dt, a, b, c, d, z, dt_bias, softplus)
-        shape = (tokens, channels)
-        _fill_rows(k.dy, dy, "dy", shape, code)
-        _fill_rows(k.dx, dx, "dx", shape, code)
-        _fill_rows(k.ddt, ddt, "ddt", shape, code)
+        tokens, channels, states, groups, sizes, rows, params = self._scan_head(x, dt, a, b, c, d, z, dt_bias, softplus)
+        shape, kind = (tokens, channels), x.dtype
         if (z is None) != (dz is None):
             raise TypeError("`dz` goes with `z`")
-        if dz is not None:
-            _fill_rows(k.dz, dz, "dz", shape, code)
-        k.db_group = _fill_runs(k.db, db, "db", tokens, groups, states, code)
-        k.dc_group = _fill_runs(k.dc, dc, "dc", tokens, groups, states, code)
-        k.da = _flat(da, "da", (channels, states), 0)
-        if dd is not None:
-            k.dd = _flat(dd, "dd", (channels,), 0)
-        if ddt_bias is not None:
-            k.ddt_bias = _flat(ddt_bias, "ddt_bias", (channels,), 0)
-        _fill_seqs(k.seqs, tokens, seq_ptr, n_seq)
-        k.state, k.dstate, k.dfinal_state = _fill_states(
-            k.seqs, (("state", state), ("dstate", dstate), ("dfinal_state", dfinal_state)), (channels, states), 0)
-        k.checkpoints, k.checkpoint_bytes = _scratch(checkpoints)
-        k.workspace, k.workspace_bytes = _scratch(workspace)
-        self._run_sequence("sparsl_dev_selective_scan_backward_device", k, "selective_scan_backward", stream)
+        dbr, dcr = _runs(db, "db", tokens, groups, states, kind), _runs(dc, "dc", tokens, groups, states, kind)
+        n, (st, ds, df) = _states((("state", state), ("dstate", dstate), ("dfinal_state", dfinal_state)),
+                                  (channels, states), 0)
+        args = _SCAN.pack(*_seqs(tokens, seq_ptr, n_seq, None, None, n), *sizes, *rows, 0, 0, *params, st, 0,
+                          *_scratch(checkpoints), *_rows(dy, "dy", shape, kind), *_rows(dx, "dx", shape, kind),
+                          *_rows(ddt, "ddt", shape, kind), *(_NONE if dz is None else _rows(dz, "dz", shape, kind)),
+                          dbr[0], dbr[1], dcr[0], dcr[1], dbr[2], dcr[2], _flat(da, "da", (channels, states), 0),
+                          _flat(dd, "dd", (channels,), 0), _flat(ddt_bias, "ddt_bias", (channels,), 0), ds, df,
+                          *_scratch(workspace))
+        self._run_sequence("sparsl_dev_selective_scan_backward_device", args, "selective_scan_backward", stream)
 
     def selective_scan_step_device(self, x, dt, a, b, c, y, state, *, d=None, z=None, dt_bias=None,
                                    softplus: bool = False, slots=None, stream=None) -> None:
         """One token of each sequence: the token arrays have a row per sequence;
         ``state`` [rows, channels, states] is updated in place.  Where
         ``slots[i]`` is negative, row i of y stays as it was."""
-        k, tokens, channels, states, groups, code = self._scan_args(x, dt, a, b, c, d, z, dt_bias, softplus)
-        _fill_rows(k.y, y, "y", (tokens, channels), code)
-        _fill_seqs(k.seqs, tokens, None, tokens, slots)
-        (k.final_state,) = _fill_states(k.seqs, (("state", state),), (channels, states), 0)
-        self._run_sequence("sparsl_dev_selective_scan_step_device", k, "selective_scan_step", stream)
+        tokens, channels, states, groups, sizes, rows, params = self._scan_head(x, dt, a, b, c, d, z, dt_bias, softplus)
+        n, (st,) = _states((("state", state),), (channels, states), 0)
+        args = _SCAN.pack(*_seqs(tokens, None, tokens, slots, None, n), *sizes, *rows,
+                          *_rows(y, "y", (tokens, channels), x.dtype), *params, 0, st,
+                          0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        self._run_sequence("sparsl_dev_selective_scan_step_device", args, "selective_scan_step", stream)
 
     # ---- layer norm ----
-    def _norm_args(self, x, weight, bias):
-        rows, channels = x.shape
-        code = _code(x, "x")
-        if code > 2:
-            raise TypeError("`x` must be float32, float16 or bfloat16")
-        a = _lib.NormArgs()
-        a.rows, a.channels, a.dtype = rows, channels, code
-        a.params_f32 = _params((("weight", weight), ("bias", bias)), ((channels,), (channels,)), code)
-        pc = 0 if a.params_f32 else code
-        _fill_rows(a.x, x, "x", (rows, channels), code)
-        if weight is not None:
-            a.weight = _flat(weight, "weight", (channels,), pc)
-        if bias is not None:
-            a.bias = _flat(bias, "bias", (channels,), pc)
-        return a, rows, channels, code
-
     def layer_norm_device(self, x, y, *, weight=None, bias=None, eps: float = 1e-5, mean=None, rstd=None,
                           stream=None) -> None:
         """y = (x - mean) rstd weight + bias over each row of ``x`` [rows, channels];
         ``mean`` and ``rstd`` [rows] float32 keep what
         :meth:`layer_norm_backward_device` needs."""
-        a, rows, channels, code = self._norm_args(x, weight, bias)
-        _fill_rows(a.y, y, "y", (rows, channels), code)
-        a.eps = eps
-        if mean is not None:
-            a.mean = _flat(mean, "mean", (rows,), 0)
-        if rstd is not None:
-            a.rstd = _flat(rstd, "rstd", (rows,), 0)
-        self._run_sequence("sparsl_dev_layer_norm_device", a, "layer_norm", stream)
+        rows, channels = shape = x.shape
+        code = _token_code(x)
+        pc = _params(weight, bias, code)
+        args = _NORM.pack(rows, channels, code, 1 if pc == 0 else 0, *_rows(x, "x", shape, x.dtype),
+                          *_rows(y, "y", shape, x.dtype), _flat(weight, "weight", (channels,), pc),
+                          _flat(bias, "bias", (channels,), pc), _flat(mean, "mean", (rows,), 0),
+                          _flat(rstd, "rstd", (rows,), 0), eps, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        self._run_sequence("sparsl_dev_layer_norm_device", args, "layer_norm", stream)
 
     @staticmethod
     def layer_norm_backward_workspace(rows: int, channels: int) -> int:
@@ -381,14 +345,12 @@ class SequenceOps:
                                    stream=None) -> None:
         """Gradients of :meth:`layer_norm_device`: ``dx`` like x, ``dweight`` and
         ``dbias`` [channels] float32, overwritten."""
-        a, rows, channels, code = self._norm_args(x, weight, None)
-        _fill_rows(a.dy, dy, "dy", (rows, channels), code)
-        _fill_rows(a.dx, dx, "dx", (rows, channels), code)
-        a.mean = _flat(mean, "mean", (rows,), 0)
-        a.rstd = _flat(rstd, "rstd", (rows,), 0)
-        if dweight is not None:
-            a.dweight = _flat(dweight, "dweight", (channels,), 0)
-        if dbias is not None:
-            a.dbias = _flat(dbias, "dbias", (channels,), 0)
-        a.workspace, a.workspace_bytes = _scratch(workspace)
-        self._run_sequence("sparsl_dev_layer_norm_backward_device", a, "layer_norm_backward", stream)
+        rows, channels = shape = x.shape
+        code = _token_code(x)
+        pc = _params(weight, None, code)
+        args = _NORM.pack(rows, channels, code, 1 if pc == 0 else 0, *_rows(x, "x", shape, x.dtype), 0, 0,
+                          _flat(weight, "weight", (channels,), pc), 0, _flat(mean, "mean", (rows,), 0),
+                          _flat(rstd, "rstd", (rows,), 0), 0.0, 0, *_rows(dy, "dy", shape, x.dtype),
+                          *_rows(dx, "dx", shape, x.dtype), _flat(dweight, "dweight", (channels,), 0),
+                          _flat(dbias, "dbias", (channels,), 0), *_scratch(workspace))
+        self._run_sequence("sparsl_dev_layer_norm_backward_device", args, "layer_norm_backward", stream)

@@ -111,6 +111,25 @@ def test_shapes_and_types_are_checked_before_the_library():
             call()
 
 
+def test_packed_blocks_fill_the_structures():
+    """Every field of a packed block lands on its structure's field of that place."""
+    import ctypes
+
+    from sparsl_b200 import sequence as Q
+
+    def flat(t, v):
+        if isinstance(v, ctypes.Structure):
+            return [w for n, f in v._fields_ for w in flat(f, getattr(v, n))]
+        return [v or 0]
+
+    for packer, struct in ((Q._CONV, _lib.ConvArgs), (Q._SCAN, _lib.ScanArgs), (Q._NORM, _lib.NormArgs)):
+        assert packer.size == ctypes.sizeof(struct)
+        count = len(packer.unpack(bytes(packer.size)))
+        values = list(range(1, count + 1))
+        got = struct.from_buffer_copy(packer.pack(*values))
+        assert flat(struct, got) == values
+
+
 def test_no_device_is_refused():
     d = _device()
     with pytest.raises(S.OpError):
