@@ -415,19 +415,19 @@ cudaError_t by_type(const ConvArgs& a, cudaStream_t s) {
 
 // Sums over the rows of part[rows, cols], each column's in one fixed order:
 // columns below `split` into out, the rest into more (null: not wanted).
-__global__ void __launch_bounds__(256) reduce_rows_kernel(const float* part, uint64_t rows, uint64_t cols,
+__global__ void __launch_bounds__(1024) reduce_rows_kernel(const float* part, uint64_t rows, uint64_t cols,
                                                           uint64_t split, float* out, float* more) {
-  __shared__ float sh[8][32];
+  __shared__ float sh[32][32];
   const uint32_t lane = threadIdx.x % 32, g = threadIdx.x / 32;
   const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
   if (c < cols)
-    for (uint64_t r = g; r < rows; r += 8) s += part[r * cols + c];
+    for (uint64_t r = g; r < rows; r += 32) s += part[r * cols + c];
   sh[g][lane] = s;
   __syncthreads();
   if (g == 0 && c < cols) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sh[k][lane];
+    for (int k = 1; k < 32; ++k) s += sh[k][lane];
     if (c < split) {
       if (out) out[c] = s;
     }
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(256) reduce_rows_kernel(const float* part, uin
 cudaError_t launch_reduce_rows(const float* part, uint64_t rows, uint64_t cols, uint64_t split, float* out, float* more,
                                cudaStream_t s) {
   if (cols == 0) return cudaSuccess;
-  reduce_rows_kernel<<<(unsigned)((cols + 31) / 32), 256, 0, s>>>(part, rows, cols, split, out, more);
+  reduce_rows_kernel<<<(unsigned)((cols + 31) / 32), 1024, 0, s>>>(part, rows, cols, split, out, more);
   return cudaGetLastError();
 }
 

@@ -38,7 +38,7 @@ cudaError_t launch_sscan_step(const SscanArgs& a, cudaStream_t s) {
 cudaError_t launch_sscan_fold_back(const float* a, const ScanWork& w, uint64_t chunks, uint32_t channels, uint32_t states,
                                    cudaStream_t s) {
   const uint64_t cells = (uint64_t)channels * states;
-  sscan_fold_kernel<true><<<(unsigned)((cells + 255) / 256), 256, 0, s>>>(a, w, chunks, channels, states);
+  sscan_fold_kernel<true><<<(unsigned)((cells + 127) / 128), 128, 0, s>>>(a, w, chunks, channels, states);
   return cudaGetLastError();
 }
 

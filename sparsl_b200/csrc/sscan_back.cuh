@@ -526,14 +526,24 @@ cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
   if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
   cudaError_t e;
   if (p.carry) {
-    // The same chunks with up to 16 states a lane: there is no history to keep.
-    constexpr int CL = NS * LP <= 16 ? 1 : NS * LP / 16, CS = NS * LP / CL;
-    ScanPlan q = p;
+    // The same chunks with up to 16 states a lane, as there is no history to keep;
+    // 4 where that leaves SMs with fewer than three blocks.
+    constexpr int NP = NS * LP, CL = NP <= 16 ? 1 : NP / 16, ML = NP <= 8 ? 2 : 4;
     const uint32_t cpg = a.channels / a.groups;
-    q.lanes = CL;
-    q.per_group = (cpg + kScanThreads / CL - 1) / (kScanThreads / CL);
-    q.ctiles = q.per_group * a.groups;
-    sscan_chunk_back_kernel<T, CS, CL, FULL, GATE><<<(unsigned)(p.chunks * q.ctiles), kScanThreads, 0, s>>>(a, q, w.scan);
+    ScanPlan q = p;
+    const auto lanes = [&](uint32_t k) {
+      q.lanes = k;
+      q.per_group = (cpg + kScanThreads / k - 1) / (kScanThreads / k);
+      q.ctiles = q.per_group * a.groups;
+      return p.chunks * q.ctiles;
+    };
+    uint64_t blocks = lanes(CL);
+    if (CL < ML && blocks < 3 * kSms) {
+      blocks = lanes(ML);
+      sscan_chunk_back_kernel<T, NP / ML, ML, FULL, GATE><<<(unsigned)blocks, kScanThreads, 0, s>>>(a, q, w.scan);
+    } else {
+      sscan_chunk_back_kernel<T, NP / CL, CL, FULL, GATE><<<(unsigned)blocks, kScanThreads, 0, s>>>(a, q, w.scan);
+    }
     e = launch_sscan_fold_back(a.a, w.scan, p.chunks, a.channels, a.states, s);
     if (e != cudaSuccess) return e;
   }

@@ -128,15 +128,15 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_chunk_kernel(Ss
 // What each chunk starts from, in place of what it hands on: ascending for the
 // states, descending (BACK) for their gradients.
 template <bool BACK>
-__global__ void __launch_bounds__(256) sscan_fold_kernel(const float* a, ScanWork w, uint64_t chunks, uint32_t channels,
+__global__ void __launch_bounds__(128) sscan_fold_kernel(const float* a, ScanWork w, uint64_t chunks, uint32_t channels,
                                                          uint32_t states) {
   const uint64_t cells = (uint64_t)channels * states;
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint64_t i = (uint64_t)blockIdx.x * 128 + threadIdx.x;
   if (i >= cells) return;
   const uint32_t c = i / states;
   const float a2 = a[i] * kLog2e;
   float carry = 0.f;
-  constexpr int U = 8;
+  constexpr int U = 16;
   for (uint64_t k = 0; k < chunks; k += U) {
     float v[U], s[U];
     int32_t cut[U];
@@ -355,9 +355,13 @@ __global__ void __launch_bounds__(kScanThreads) sscan_step_kernel(SscanArgs a, u
 // used.  A lane of 4 states took 200 instructions a token, for the step, the
 // gate and the addresses over again in each: 84 us against HBM's 44 for 512
 // tokens x 4096 channels x 16 states.
-constexpr int kStepTokens = 4;
+#ifndef STEP_TOK
+#define STEP_TOK 2
+#define STEP_RES 6
+#endif
+constexpr int kStepTokens = STEP_TOK;
 template <class T, int NS, int LP, bool FULL>
-__global__ void __launch_bounds__(kScanThreads, kResident) sscan_step_many_kernel(SscanArgs a, uint32_t per_group, uint32_t ctiles) {
+__global__ void __launch_bounds__(kScanThreads, STEP_RES) sscan_step_many_kernel(SscanArgs a, uint32_t per_group, uint32_t ctiles) {
   constexpr int NP = NS * LP;
   __shared__ __align__(16) float bc[kStepTokens][2][NP];
   const uint32_t N = a.states;
@@ -429,7 +433,7 @@ cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
   if (p.carry) {
     sscan_chunk_kernel<T, NS, LP, FULL><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w, aligned);
     const uint64_t cells = (uint64_t)a.channels * a.states;
-    sscan_fold_kernel<false><<<(unsigned)((cells + 255) / 256), 256, 0, s>>>(a.a, w, p.chunks, a.channels, a.states);
+    sscan_fold_kernel<false><<<(unsigned)((cells + 127) / 128), 128, 0, s>>>(a.a, w, p.chunks, a.channels, a.states);
   }
   if (a.z) sscan_kernel<T, NS, LP, FULL, true><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w, aligned);
   else sscan_kernel<T, NS, LP, FULL, false><<<(unsigned)grid, kScanThreads, 0, s>>>(a, p, w, aligned);
