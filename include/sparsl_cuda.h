@@ -432,8 +432,8 @@ int sparsl_dev_assoc_scan_noalloc(int ordinal, const float *d_in, uint64_t n, fl
  *  - slots (device, n_seq): the row of the state arrays that sequence i uses;
  *    NULL: row i.  A slot outside [0, n_slots) is none: the sequence starts
  *    from zero and leaves no state (in a step, its row is skipped).  Two
- *    sequences of a call must not name the same slot: which of them it then
- *    holds is not specified.
+ *    sequences of a call must not name the same slot: its values are then not
+ *    specified.
  *  - state: what each sequence starts from; NULL: zeros.  resume (device,
  *    n_seq bytes): a 0 starts that sequence from zero instead; NULL: all
  *    resume.  final_state: where its state behind the last token goes, also

@@ -237,6 +237,28 @@ __device__ __forceinline__ void store_pairs(float* p, uint32_t n0, uint32_t N, c
   for (int j = 0; j < NS / 2; ++j) unpair(h[j], v[2 * j], v[2 * j + 1]);
   store_states<NS, FULL>(p, n0, N, v);
 }
+// The same 32 bytes at a time, a whole sector of a lane's row by one instruction
+// (FULL, NS a multiple of 8, rows on 32-byte boundaries).
+template <int NS, bool FULL>
+__device__ __forceinline__ void load_rows(const float* p, uint32_t n0, uint32_t N, f32x2 (&h)[NS / 2]) {
+  if constexpr (FULL && NS % 8 == 0) {
+#pragma unroll
+    for (int j = 0; j < NS / 2; j += 4)
+      asm volatile("ld.global.v4.b64 {%0, %1, %2, %3}, [%4];" : "=l"(h[j]), "=l"(h[j + 1]), "=l"(h[j + 2]), "=l"(h[j + 3]) : "l"(p + n0 + 2 * j) : "memory");
+  } else {
+    load_pairs<NS, FULL>(p, n0, N, h);
+  }
+}
+template <int NS, bool FULL>
+__device__ __forceinline__ void store_rows(float* p, uint32_t n0, uint32_t N, const f32x2 (&h)[NS / 2]) {
+  if constexpr (FULL && NS % 8 == 0) {
+#pragma unroll
+    for (int j = 0; j < NS / 2; j += 4)
+      asm volatile("st.global.v4.b64 [%0], {%1, %2, %3, %4};" ::"l"(p + n0 + 2 * j), "l"(h[j]), "l"(h[j + 1]), "l"(h[j + 2]), "l"(h[j + 3]) : "memory");
+  } else {
+    store_pairs<NS, FULL>(p, n0, N, h);
+  }
+}
 template <int M>
 __device__ __forceinline__ void zero_pairs(f32x2 (&h)[M]) {
 #pragma unroll

@@ -522,8 +522,8 @@ template <class T, int NS, int LP, bool FULL, bool GATE>
 cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
   BackWork w{};
   back_work(p, a.seq.tokens, a.channels, a.states, a.groups, a.work, &w);
-  const uint64_t grid = p.chunks * p.ctiles;
-  if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
+  const uint64_t grid = p.chunks * p.ctiles, cells = a.seq.tokens * a.groups * 2 * a.states;
+  if (grid > 0x7fffffffull / 8 || cells / 256 >= 0x7fffffffull) return cudaErrorInvalidValue;
   cudaError_t e;
   if (p.carry) {
     // The same chunks with up to 16 states a lane, as there is no history to keep;
@@ -556,7 +556,6 @@ cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
   const int aligned = rows_aligned<T, LP>(a, {{a.x, a.x_row}, {a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row},
                                               {a.dx, a.dx_row}, {a.ddt, a.ddt_row}, {a.dz, a.dz_row}});
   kernel<<<(unsigned)grid, kScanThreads, bytes, s>>>(a, p, w, aligned);
-  const uint64_t cells = a.seq.tokens * a.groups * 2 * a.states;
   if (cells) sscan_bc_kernel<T><<<(unsigned)((cells + 255) / 256), 256, 0, s>>>(a, w.bc, p.per_group);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;

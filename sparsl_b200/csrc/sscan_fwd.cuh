@@ -352,16 +352,12 @@ __global__ void __launch_bounds__(kScanThreads) sscan_step_kernel(SscanArgs a, u
 
 // Many sequences: up to 16 states a lane, as in the scan, and a block's channels
 // for kStepTokens of them, whose states are all asked for before the first is
-// used.  A lane of 4 states took 200 instructions a token, for the step, the
-// gate and the addresses over again in each: 84 us against HBM's 44 for 512
-// tokens x 4096 channels x 16 states.
-#ifndef STEP_TOK
-#define STEP_TOK 2
-#define STEP_RES 6
-#endif
-constexpr int kStepTokens = STEP_TOK;
+// used, 32 bytes an access.  512 tokens x 4096 channels x 16 states: 57 us, 5.0
+// TB/s of states and rows; with 4 states a lane 77 us, the step, the gate and the
+// addresses over again in each, and with 16-byte accesses, half a sector each, 67.
+constexpr int kStepTokens = 4;
 template <class T, int NS, int LP, bool FULL>
-__global__ void __launch_bounds__(kScanThreads, STEP_RES) sscan_step_many_kernel(SscanArgs a, uint32_t per_group, uint32_t ctiles) {
+__global__ void __launch_bounds__(kScanThreads, kResident) sscan_step_many_kernel(SscanArgs a, uint32_t per_group, uint32_t ctiles) {
   constexpr int NP = NS * LP;
   __shared__ __align__(16) float bc[kStepTokens][2][NP];
   const uint32_t N = a.states;
@@ -375,7 +371,7 @@ __global__ void __launch_bounds__(kScanThreads, STEP_RES) sscan_step_many_kernel
     const int64_t i = i0 + u, slot = i < (int64_t)a.seq.n_seq ? a.seq.slot(i) : -1;
     at[u] = slot < 0 ? -1 : (int64_t)(((uint64_t)slot * a.channels + me.c) * N);
     if (at[u] < 0) continue;  // the whole block's
-    load_pairs<NS, FULL>(a.final_state + at[u], me.n0, N, h[u]);
+    load_rows<NS, FULL>(a.final_state + at[u], me.n0, N, h[u]);
     xv[u] = to_f32(*cell<T>(a.x, i, a.x_row, me.c));
     s[u] = to_f32(*cell<T>(a.dt, i, a.dt_row, me.c));
     zv[u] = a.z ? to_f32(*cell<T>(a.z, i, a.z_row, me.c)) : 0.f;
@@ -404,7 +400,7 @@ __global__ void __launch_bounds__(kScanThreads, STEP_RES) sscan_step_many_kernel
     o = __fmaf_rn(dskip, xv[u], o);
     if (a.z) o *= zv[u] * sigmoid(zv[u]);
     if (!me.valid) continue;
-    store_pairs<NS, FULL>(a.final_state + at[u], me.n0, N, h[u]);
+    store_rows<NS, FULL>(a.final_state + at[u], me.n0, N, h[u]);
     if (me.first) *cell<T>(a.y, i0 + u, a.y_row, me.c) = from_f32<T>(o);
   }
 }
@@ -493,15 +489,16 @@ template <class T>
 cudaError_t step_by_states(const SscanArgs& a, cudaStream_t s) {
   const uint32_t N = a.states;
   const bool al = aligned16(a.a) && aligned16(a.final_state);
+  const bool wide = aligned16(a.a) && reinterpret_cast<uint64_t>(a.final_state) % 32 == 0;
   uint32_t per;
   uint64_t grid;
-  if (N <= 8 && many<1>(a, per, grid)) return N == 8 && al ? go_many<T, 8, 1, true>(a, per, grid, s) : go_many<T, 8, 1, false>(a, per, grid, s);
+  if (N <= 8 && many<1>(a, per, grid)) return N == 8 && wide ? go_many<T, 8, 1, true>(a, per, grid, s) : go_many<T, 8, 1, false>(a, per, grid, s);
   if (N > 8 && N <= 16 && many<1>(a, per, grid))
-    return N == 16 && al ? go_many<T, 16, 1, true>(a, per, grid, s) : go_many<T, 16, 1, false>(a, per, grid, s);
+    return N == 16 && wide ? go_many<T, 16, 1, true>(a, per, grid, s) : go_many<T, 16, 1, false>(a, per, grid, s);
   if (N > 16 && N <= 32 && many<2>(a, per, grid))
-    return N == 32 && al ? go_many<T, 16, 2, true>(a, per, grid, s) : go_many<T, 16, 2, false>(a, per, grid, s);
+    return N == 32 && wide ? go_many<T, 16, 2, true>(a, per, grid, s) : go_many<T, 16, 2, false>(a, per, grid, s);
   if (N > 32 && many<4>(a, per, grid))
-    return N == 64 && al ? go_many<T, 16, 4, true>(a, per, grid, s) : go_many<T, 16, 4, false>(a, per, grid, s);
+    return N == 64 && wide ? go_many<T, 16, 4, true>(a, per, grid, s) : go_many<T, 16, 4, false>(a, per, grid, s);
   if (N == 16 && al) return go_step<T, 4, true>(a, s);
   if (N == 8 && al) return go_step<T, 2, true>(a, s);
   if (N == 32 && al) return go_step<T, 8, true>(a, s);

@@ -250,6 +250,46 @@ def test_scan_tokens_one_by_one(cuda_device, ns, dtype):
     assert torch.equal(pool[rest], before[rest])
 
 
+@pytest.mark.parametrize("ns", [16, 8, 5, 20, 40, 64])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_scan_tokens_of_many_sequences(cuda_device, ns, dtype):
+    """A batch large enough for the kernel that takes several sequences a block; some have no state."""
+    n, ch = 603, 514
+    s = Scan([1] * n, ch, ns, 2, dtype, state=True, ragged=False)
+    slots = torch.randperm(n + 7, generator=_gen(ns))[:n].to(torch.int32)
+    slots[[3, 4, 100, 602]] = -1
+    rows = slots.tolist()
+    pool = torch.full((n + 7, ch, ns), 3.0, device="cuda")
+    live = torch.tensor([i for i, r in enumerate(rows) if r >= 0])
+    pool[slots[live].long()] = s.state[live.cuda()]
+    before = pool.clone()
+    y = torch.full((n, ch), 7.0, dtype=dtype, device="cuda")
+    cuda_device.selective_scan_step_device(s.x, s.dt, s.a, s.b, s.c, y, pool, d=s.d, z=s.z, dt_bias=s.bias, softplus=True,
+                                           slots=slots.cuda(), stream=_stream())
+    want, k = s.oracle(s.state)
+    R.check(y[live.cuda()], want["y"][0][live], want["y"][1][live], k, "y")
+    R.check(pool[slots[live].long()], want["final"][0][live], want["final"][1][live], k, "state")
+    assert (y[[3, 4, 100, 602]] == 7).all()
+    rest = [r for r in range(n + 7) if r not in rows]
+    assert torch.equal(pool[rest], before[rest])
+
+
+@pytest.mark.parametrize("shape", [dict(lens=[1] * 333, ch=40, ns=16, tail=3), dict(lens=[2, 1, 3] * 60, ch=17, ns=8, lead=9),
+                                   dict(lens=[64] * 40, ch=260, ns=16, ragged=False), dict(lens=[32] * 9, ch=1200, ns=4, ragged=False),
+                                   dict(lens=[96] * 12, ch=384, ns=32, ragged=False, groups=2)], ids=str)
+def test_scan_many_sequences(cuda_device, shape):
+    s = Scan(state=True, dtype=torch.bfloat16, **shape)
+    marks = s.marks(cuda_device)
+    want, k = s.oracle(s.state, backward=True)
+    final = torch.full_like(s.state, NAN)
+    y = s.forward(cuda_device, marks=marks, state=s.state, final=final)
+    R.check(s.live(y), *want["y"], k, "y")
+    R.check(final, *want["final"], k, "final")
+    s.untouched(y)
+    for name, v in s.backward(cuda_device, marks).items():
+        R.check(s.live(v) if name in ("dx", "ddt", "db", "dc", "dz") else v, *want[name], k, name)
+
+
 def test_scan_infinite_and_nan_stay_in_their_sequence(cuda_device):
     s = Scan([50, 40, 60], 20, 11)
     clean = s.forward(cuda_device)
@@ -451,7 +491,8 @@ def test_conv_tokens_one_by_one(cuda_device, ch, dtype, width):
 # ---- layer norm ------------------------------------------------------------------------------------
 
 NORMS = [(1, 1), (3, 2), (5, 31), (2, 32), (7, 33), (1000, 100), (4, 1024), (3, 1030), (300, 520), (2, 4096), (700, 2048), (9, 5003),
-         (400, 8192), (3, 8200), (2, 16384), (301, 12001), (2, 33000), (0, 64)]
+         (400, 8192), (3, 8200), (2, 16384), (301, 12001), (2, 33000), (0, 64),
+         (2400, 104), (2369, 520), (2371, 1032), (2370, 2048), (2368, 4000), (2380, 6144), (2369, 8192), (2400, 33)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
