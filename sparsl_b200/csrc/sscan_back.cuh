@@ -319,6 +319,11 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
       const auto walk = [&](auto edges) {
         constexpr bool EDGES = decltype(edges)::value;
         f32x2 hp[K][NH], e[NH], en[NH];
+        // This block's sums over tokens, added to the chunk's at its end: one running sum over
+        // the thousands of tokens of a chunk loses a decimal place to a sum of sums.
+        f32x2 da_block[NH];
+        float dd_block = 0.f, dbias_block = 0.f;
+        zero_pairs(da_block);
         float o[LP];
         // Forwards.
         float4 now = cells[0], next;
@@ -404,7 +409,7 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
               r[i + u] = mul2(e[i + u], gh);
               const f32x2 through = mul2(r[i + u], hp[k][i + u]);
               ga2 = fma2(through, a2[i + u], ga2);
-              da[i + u] = fma2(through, ss, da[i + u]);
+              da_block[i + u] = fma2(through, ss, da_block[i + u]);
               v[i + u] = mul2(gh, xx);
             }
           }
@@ -415,8 +420,8 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
           if (q == 0) {
             const float gbs = scatter_sum<LP>(gb, part), gas = scatter_sum<LP>(ga, part);
             const float ds = (live >> (j * LP + part) & 1) ? __fmaf_rn(gas, 1.0f / kLog2e, xv[j] * gbs) * slope[j] : 0.f;
-            dd = __fmaf_rn(g[j], xv[j], dd);
-            dbias += ds;
+            dd_block = __fmaf_rn(g[j], xv[j], dd_block);
+            dbias_block += ds;
             result[0][j * LP + part][col] = from_f32<T>(__fmaf_rn(dskip, g[j], s[j] * gbs));
             result[1][j * LP + part][col] = from_f32<T>(ds);
           }
@@ -429,6 +434,10 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
           for (int i = 0; i < NH; ++i) e[i] = en[i];
           now = next;
         }
+#pragma unroll
+        for (int i = 0; i < NH; ++i) da[i] = add2(da[i], da_block[i]);
+        dd += dd_block;
+        dbias += dbias_block;
       };
       if (live == kAll && !(start & ~1u) && !(end & (kAll >> 1))) walk(std::false_type{});
       else if (live) walk(std::true_type{});

@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kScanThreads) sscan_step_kernel(SscanArgs a, u
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (FULL || n0 + j < N) {
-      h[j] = __fmaf_rn(ex2(s * (a2[j] * kLog2e)), h[j], s * xv * to_f32(b[n0 + j]));
+      h[j] = __fmaf_rn(ex2(__fmaf_rn(s, a2[j] * kLog2e, kLift)), h[j], s * xv * to_f32(b[n0 + j]));
       o = __fmaf_rn(to_f32(cv[n0 + j]), h[j], o);
     }
   }
