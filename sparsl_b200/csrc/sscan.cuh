@@ -401,6 +401,44 @@ struct WarpRows {
     }
   }
 };
+// The pieces of aligned rows that a lane copies for each batch, batch after batch
+// (DIR 1) or back from the last (DIR -1): where they are, kept and moved on, as
+// their addresses from scratch took as long as a token's arithmetic.
+template <class T, int LP, int A, int DIR>
+struct RowsCursor {
+  using Rows = WarpRows<T, LP>;
+  static constexpr int kN = (A * Rows::kLanes + 31) / 32;
+  const char* from[kN];
+  uint32_t bytes[kN];  // of the piece that exist; 0: none
+  int32_t row[kN];
+  __device__ __forceinline__ RowsCursor(const RowsIn (&r)[A], int64_t t, uint32_t c0, uint32_t cols) {
+#pragma unroll
+    for (int it = 0; it < kN; ++it) {
+      const uint32_t i = it * 32 + (threadIdx.x & 31), piece = i % Rows::kPieces, k = i / Rows::kPieces % kBatch;
+      // Whole iterations are one array's: known when compiled.
+      const uint32_t which = Rows::kLanes % 32 == 0 ? it * 32 / Rows::kLanes : i / Rows::kLanes;
+      RowsIn s = r[0];
+#pragma unroll
+      for (int q = 1; q < A; ++q)
+        if (which == (uint32_t)q) s = r[q];
+      const uint32_t first = piece * Rows::kPiece, have = cols * (uint32_t)sizeof(T);
+      bytes[it] = which >= (uint32_t)A || have <= first ? 0 : have - first < Rows::kPiece ? have - first : Rows::kPiece;
+      row[it] = (int32_t)s.row;
+      from[it] = static_cast<const char*>(s.p) + ((t + (int64_t)k) * (int64_t)row[it] + (int64_t)c0 * (int64_t)sizeof(T) + first);
+    }
+  }
+  __device__ __forceinline__ void copy(T (*to)[kBatch][Rows::kCols], uint32_t live) {
+    char* const base = reinterpret_cast<char*>(&to[0][0][0]) + (threadIdx.x & 31) * Rows::kPiece;
+    const uint32_t k0 = (threadIdx.x & 31) / Rows::kPieces;
+#pragma unroll
+    for (int it = 0; it < kN; ++it) {
+      const uint32_t k = (it * (32 / Rows::kPieces) + k0) % kBatch;
+      if (bytes[it] && (live >> k & 1)) copy_async<Rows::kPiece>(base + it * 32 * Rows::kPiece, from[it], bytes[it]);
+      from[it] += (int64_t)row[it] * (DIR * kBatch);
+    }
+  }
+};
+
 // 2 where the pieces of a warp's channels start on their own size in every row,
 // 1 where they start on 4 bytes.
 template <class T, int LP>

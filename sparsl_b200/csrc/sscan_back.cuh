@@ -47,9 +47,11 @@ __device__ __forceinline__ float gate_grad(float z, float sig) { return sig * __
 // sequence that reaches into it, or from zero at its own end; in batches of
 // eight tokens, the last ones first.
 template <class T, int NS, int LP, bool FULL, bool GATE>
-__global__ void __launch_bounds__(kScanThreads, 4) sscan_chunk_back_kernel(SscanArgs a, ScanPlan p, ScanWork w) {
-  constexpr int NP = NS * LP, U = 8, kOwn = U / LP;
+__global__ void __launch_bounds__(kScanThreads, 4) sscan_chunk_back_kernel(SscanArgs a, ScanPlan p, ScanWork w, int aligned) {
+  constexpr int NP = NS * LP, U = kBatch, kOwn = U / LP, A = GATE ? 3 : 2;
+  using Rows = WarpRows<T, LP>;
   __shared__ __align__(16) float sc[2][kScanTile][NP];
+  __shared__ __align__(16) T rows[kScanThreads / 32][2][A][U][Rows::kCols];
   const uint32_t N = a.states;
   const ScanLane<NS, LP> me(a.channels, a.groups, p.per_group, blockIdx.x % p.ctiles);
   const uint32_t part = threadIdx.x % LP;
@@ -70,59 +72,61 @@ __global__ void __launch_bounds__(kScanThreads, 4) sscan_chunk_back_kernel(Sscan
     if (slot >= 0) load_pairs<NS, FULL>(a.dfinal + ((uint64_t)slot * a.channels + me.c) * N, me.n0, N, r);
   }
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
-  const T* dt = reinterpret_cast<const T*>(a.dt) + me.c;
-  const T* dy = reinterpret_cast<const T*>(a.dy) + me.c;
-  const T* z = GATE ? reinterpret_cast<const T*>(a.z) + me.c : nullptr;
+  const uint32_t col = threadIdx.x % 32 / LP;
   float sum = 0.f;
-  T dr[kOwn], gr[kOwn], zr[kOwn];
-  const auto load = [&](int64_t te) {  // own tokens of the batch that ends in front of te
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) {
-      const int64_t t = te - 1 - (j * LP + (int64_t)part);
-      if (t < t0) continue;
-      dr[j] = dt[(uint64_t)t * a.dt_stride];
-      gr[j] = dy[(uint64_t)t * a.dy_stride];
-      if (GATE) zr[j] = z[(uint64_t)t * a.z_stride];
-    }
+  RowsIn arrays[A];
+  arrays[0] = {a.dt, a.dt_row};
+  arrays[1] = {a.dy, a.dy_row};
+  if constexpr (GATE) arrays[2] = {a.z, a.z_row};
+  T(*const stages)[A][U][Rows::kCols] = rows[threadIdx.x / 32];
+  RowsCursor<T, LP, A, -1> cursor(arrays, hi - U, me.warp_c, me.warp_cols);
+  // The bits of tokens t.. that the chunk has.
+  const auto above = [&](int64_t t) { return t >= t0 ? ~0u : ~first_bits(t0 - t); };
+  const auto fetch = [&](int at, int64_t t) {
+    if (aligned == 2) cursor.copy(stages[at], above(t));
+    else Rows::in(stages[at], arrays, t, above(t), me.warp_c, me.warp_cols, aligned);
+    copies_issued();
   };
   StageBC<T, NP, 1, true> stage;
-  const auto above = [&](int64_t tb) { return tb >= t0 ? ~0u : ~first_bits(t0 - tb); };
   stage.fetch(a, me.group, hi - kScanTile, above(hi - kScanTile));
+  fetch(0, hi - U);
   stage.put(&sc[0][0][0]);
-  load(hi);
   __syncthreads();
-  int buf = 0;
-  for (int64_t te = hi; te > t0; te -= kScanTile, buf ^= 1) {
+  int buf = 0, at = 0;
+  for (int64_t te = hi; te > t0; te -= kScanTile, buf ^= 1) {  // tokens te - 32 to te - 1, the last first
     stage.fetch(a, me.group, te - 2 * kScanTile, above(te - 2 * kScanTile));
 #pragma unroll 1
-    for (int k0 = 0; k0 < kScanTile; k0 += U) {
-      const int64_t left = te - k0 - t0;
-      if (left <= 0) break;
+    for (int k0 = 0; k0 < kScanTile; k0 += U, at ^= 1) {
+      const int64_t tb = te - k0 - U;  // the batch's first token
+      if (tb + U <= t0) break;
+      copies_done();
+      fetch(at ^ 1, tb - U);
+      const T(&in)[A][U][Rows::kCols] = stages[at];
+      const uint32_t live = above(tb);
       float s[kOwn], g[kOwn];
 #pragma unroll
       for (int j = 0; j < kOwn; ++j) {
-        const bool live = j * LP + (int64_t)part < left;
-        s[j] = g[j] = 0.f;  // a token in front of the chunk changes nothing: e = 1
-        if (live) {
-          s[j] = to_f32(dr[j]) + bias;
+        const int k = j * LP + part;
+        s[j] = g[j] = 0.f;  // a token in front of the chunk changes nothing: its decay is 1
+        if (live >> k & 1) {
+          s[j] = to_f32(in[0][k][col]) + bias;
           if (a.softplus) s[j] = softplus(s[j]);
           sum += s[j];
-          g[j] = to_f32(gr[j]);
+          g[j] = to_f32(in[1][k][col]);
           if (GATE) {
-            const float zv = to_f32(zr[j]);
+            const float zv = to_f32(in[A - 1][k][col]);
             g[j] *= zv * sigmoid(zv);
           }
         }
       }
-      load(te - k0 - U);
       f32x2 e[NS / 2], en[NS / 2];
-      decay<NS>(from_lane<LP>(s[0], 0), a2, e);
+      decay<NS>(from_lane<LP>(s[kOwn - 1], LP - 1), a2, e);
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        if (k + 1 < U) decay<NS>(from_lane<LP>(s[(k + 1) / LP], (k + 1) % LP), a2, en);
+      for (int k = U - 1; k >= 0; --k) {
+        if (k) decay<NS>(from_lane<LP>(s[(k ? k - 1 : 0) / LP], (k ? k - 1 : 0) % LP), a2, en);
         const float gv = from_lane<LP>(g[k / LP], k % LP);
         const f32x2 gg = pair(gv, gv);
-        const float* row = &sc[buf][kScanTile - 1 - (k0 + k)][me.n0];
+        const float* row = &sc[buf][kScanTile - U - k0 + k][me.n0];
 #pragma unroll
         for (int i = 0; i < NS / 2; i += 2) {
           const ulonglong2 cc = *reinterpret_cast<const ulonglong2*>(row + 2 * i);
@@ -242,8 +246,11 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
   arrays[1] = {a.dt, a.dt_row};
   arrays[2] = {a.dy, a.dy_row};
   if constexpr (GATE) arrays[3] = {a.z, a.z_row};
+  const int64_t tiles = (t1 - t0 + kScanTile - 1) / kScanTile;
+  RowsCursor<T, LP, A, -1> cursor(arrays, t0 + tiles * kScanTile - K, me.warp_c, me.warp_cols);
   const auto fetch = [&](int at, int64_t t, uint32_t live) {
-    Rows::in(sh.rows[warp][at], arrays, t, live, me.warp_c, me.warp_cols, aligned);
+    if (aligned == 2) cursor.copy(sh.rows[warp][at], live);
+    else Rows::in(sh.rows[warp][at], arrays, t, live, me.warp_c, me.warp_cols, aligned);
     if (live & 1) {
       const float* from = a.marks + ((uint64_t)(t / K) * a.channels + me.warp_c) * N;
       float* to = &sh.mark[warp][at][0][0];
@@ -263,7 +270,6 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
   float* const part_rows = w.bc + ((uint64_t)me.channel_tile * a.seq.tokens * a.groups + me.group) * 2 * N;
   const uint32_t part_row = a.groups * 2 * N;
 
-  const int64_t tiles = (t1 - t0 + kScanTile - 1) / kScanTile;
   StageBC<T, NP, 2> stage;
   TileMarks m, before;
   if (tiles > 0) {
@@ -549,9 +555,11 @@ cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
     uint64_t blocks = lanes(CL);
     if (CL < ML && blocks < 3 * kSms) {
       blocks = lanes(ML);
-      sscan_chunk_back_kernel<T, NP / ML, ML, FULL, GATE><<<(unsigned)blocks, kScanThreads, 0, s>>>(a, q, w.scan);
+      sscan_chunk_back_kernel<T, NP / ML, ML, FULL, GATE><<<(unsigned)blocks, kScanThreads, 0, s>>>(
+          a, q, w.scan, rows_aligned<T, ML>(a, {{a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row}}));
     } else {
-      sscan_chunk_back_kernel<T, NP / CL, CL, FULL, GATE><<<(unsigned)blocks, kScanThreads, 0, s>>>(a, q, w.scan);
+      sscan_chunk_back_kernel<T, NP / CL, CL, FULL, GATE><<<(unsigned)blocks, kScanThreads, 0, s>>>(
+          a, q, w.scan, rows_aligned<T, CL>(a, {{a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row}}));
     }
     e = launch_sscan_fold_back(a.a, w.scan, p.chunks, a.channels, a.states, s);
     if (e != cudaSuccess) return e;

@@ -76,8 +76,10 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_chunk_kernel(Ss
   const int64_t from = max(begin, t0);
   const RowsIn arrays[2] = {{a.x, a.x_row}, {a.dt, a.dt_row}};
   T(*const stages)[2][K][Rows::kCols] = rows[threadIdx.x / 32];
+  RowsCursor<T, LP, 2, 1> cursor(arrays, from, me.warp_c, me.warp_cols);
   const auto fetch = [&](int at, int64_t t) {
-    Rows::in(stages[at], arrays, t, first_bits(t1 - t), me.warp_c, me.warp_cols, aligned);
+    if (aligned == 2) cursor.copy(stages[at], first_bits(t1 - t));
+    else Rows::in(stages[at], arrays, t, first_bits(t1 - t), me.warp_c, me.warp_cols, aligned);
     copies_issued();
   };
   stage.fetch(a, me.group, from, first_bits(t1 - from));
@@ -224,8 +226,10 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArg
   if constexpr (GATE) arrays[2] = {a.z, a.z_row};
   T(*const stages)[A][K][Rows::kCols] = rows[threadIdx.x / 32];
   T(&result)[K][Rows::kCols] = results[threadIdx.x / 32];
+  RowsCursor<T, LP, A, 1> cursor(arrays, t0, me.warp_c, me.warp_cols);
   const auto fetch = [&](int at, int64_t t, uint32_t live) {
-    Rows::in(stages[at], arrays, t, live, me.warp_c, me.warp_cols, aligned);
+    if (aligned == 2) cursor.copy(stages[at], live);
+    else Rows::in(stages[at], arrays, t, live, me.warp_c, me.warp_cols, aligned);
     copies_issued();
   };
   StageBC<T, NP, 2> stage;
