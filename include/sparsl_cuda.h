@@ -30,7 +30,8 @@
  *  - Precision: 0 = f32, 1 = binary16, 2 = bfloat16 (WeightPrecision,
  *    src/backend/mod.rs:588-652).  The library quantises exactly as
  *    WeightPrecision::quantise (mod.rs:624-641) with the half.rs encoders.
- *  - Every floating-point result is bit-identical to the reference's
+ *  - Every floating-point result of the reference's operations (all but the
+ *    sequence operators, which it has not) is bit-identical to the reference's
  *    CpuSequential arm on the same inputs (NaN payloads excepted; NaN class is
  *    preserved), because every output is one strict left fold with separate
  *    round-to-nearest multiply and add, as in mod.rs:2259-2267.

@@ -642,6 +642,48 @@ def test_other_streams(cuda_device):
     assert torch.equal(y1, y2) and torch.equal(y1, y3)
 
 
+def test_two_threads_at_once(cuda_device):
+    """Calls from two threads, each on its own stream with its own arrays, give what they give alone."""
+    import threading
+
+    sets = [Scan([120, 33, 70], 64, 16, dtype=torch.bfloat16, state=True, seed=k) for k in (21, 22)]
+    marks = [s.marks(cuda_device) for s in sets]
+    alone = [(s.forward(cuda_device, marks=m, state=s.state), s.backward(cuda_device, m)) for s, m in zip(sets, marks)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(s, m, want):
+        try:
+            side = torch.cuda.Stream()
+            with torch.cuda.stream(side):
+                for _ in range(10):
+                    y = s.forward(cuda_device, marks=m, state=s.state, stream=side)
+                    got = s.backward(cuda_device, m, stream=side)
+            side.synchronize()
+            assert torch.equal(y, want[0]) and all(torch.equal(v, want[1][k]) for k, v in got.items())
+        except Exception as e:  # noqa: BLE001 (reported by the main thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(sets, marks, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
+def test_current_device_is_kept(cuda_device):
+    """A call leaves the thread's current device and its torch stream as they were, and nothing allocated."""
+    s = Scan([64], 32, 16, ragged=False)
+    y, room = torch.zeros_like(s.x), _room(cuda_device.selective_scan_workspace(64, 32, 16, 1, 1))
+    torch.cuda.synchronize()
+    before = (torch.cuda.current_device(), torch.cuda.mem_get_info()[0], torch.cuda.memory_allocated())
+    for _ in range(3):
+        cuda_device.selective_scan_device(s.x, s.dt, s.a, s.b, s.c, y, room, stream=_stream())
+    torch.cuda.synchronize()
+    assert before == (torch.cuda.current_device(), torch.cuda.mem_get_info()[0], torch.cuda.memory_allocated())
+
+
 def test_sequence_starts_outside_the_tokens_are_clamped(cuda_device):
     """No content of seq_ptr or slots leads an access out of the arrays: their neighbours stay as they are."""
     s, v = Scan([40, 30, 26], 20, 16, state=True), Conv([40, 30, 26], 20, 4, state=True)
