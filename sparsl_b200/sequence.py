@@ -17,6 +17,7 @@ from . import _lib
 
 _CODES = {}  # dtype -> sparsl dtype code, for those seen
 _KINDS = {0: "float32", 1: "float16", 2: "bfloat16", 10: "int32", 11: "uint8"}
+_CALLS = {}  # the library's entries, for those called
 _NONE = (0, 0)  # no rows
 
 
@@ -156,7 +157,10 @@ class SequenceOps:
     """Mixed into ``Device``."""
 
     def _run_sequence(self, fn: str, args: bytes, operation: str, stream):
-        rc = getattr(_lib.load(), fn)(self._h, args, _stream(stream))
+        call = _CALLS.get(fn)
+        if call is None:
+            call = _CALLS[fn] = getattr(_lib.load(), fn)
+        rc = call(self._h, args, _stream(stream))
         if rc:
             from .backend import _check
 
