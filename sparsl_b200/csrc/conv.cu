@@ -311,8 +311,8 @@ __global__ void __launch_bounds__(kThreads) conv_backward_kernel(ConvArgs a, uin
 #pragma unroll
           for (int m = 0; m < W; ++m) g[j] = __fmaf_rn(w[W - 1 - m][j], du.v[m][j], g[j]);
         }
-        const int64_t fr = s - (end - (W - 1));  // its row in the final state
-        if (df && fr >= 0) {
+        const int64_t fr = s - (end - (W - 1));  // its row in the final state; behind it where seq_ptr does not ascend
+        if (df && fr >= 0 && fr < W - 1) {
           float f[V];
           load_pack<T, V>(df + (uint64_t)fr * a.channels, f);
 #pragma unroll

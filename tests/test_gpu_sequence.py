@@ -705,6 +705,24 @@ def test_sequence_starts_outside_the_tokens_are_clamped(cuda_device):
             assert (t == 5).all()
 
 
+def test_conv_gradients_of_starts_that_do_not_ascend(cuda_device):
+    """A sequence that begins and ends in front of what its tile has done reads no row behind its final state's gradient;
+    the outputs' neighbours stay as they are."""
+    for ptr in ([23, 22, 15, 18, 17, 2, 0, 30], [40, 30, 0, 17, 16, 16, 40], [16, 31, 20, 24, 16, 18, 32, 17]):
+        n = len(ptr) - 1
+        v = Conv([40] + [0] * (n - 1), 33, 4, state=True)
+        v.ptr = torch.tensor(ptr, dtype=torch.int32).cuda()
+        guard = torch.full((n + 2, 3, 33), 5.0, device="cuda")
+        dx = torch.full((44, 33), 5.0, device="cuda")
+        dw, room = torch.zeros_like(v.w), _room(cuda_device.causal_conv_backward_workspace(40, 33, 4))
+        cuda_device.causal_conv_backward_device(v.dy, v.x, v.w, dx[2:-2], dw, room, bias=v.bias, silu=True, seq_ptr=v.ptr,
+                                                state=v.state, dstate=guard[1:-1], dfinal_state=v.dfinal, stream=_stream())
+        torch.cuda.synchronize()
+        for t in (guard[:1], guard[-1:], dx[:2], dx[-2:]):
+            assert (t == 5).all()
+        assert torch.isfinite(dw).all()
+
+
 def _refused(kind, call, *args, **kw):
     with pytest.raises(OpError) as e:
         call(*args, **kw)
