@@ -498,7 +498,8 @@ int sparsl_dev_causal_conv_step_device(sparsl_dev *dev, const sparsl_conv_args *
  * y = sum_n c[n] h[c, n] + d[c] x, times z sigmoid(z) with z.
  * a [channels, states], d, dt_bias [channels] or NULL: f32.  b, c: per token
  * `groups` runs of `states` values (a run every b_group / c_group elements);
- * channels / groups neighbouring channels share a run.  states 1..64.
+ * channels / groups neighbouring channels share a run.  states 1..64.  Rows of
+ * x, dt, z, y and their gradients lie less than 2^29 elements apart.
  * state, final_state and their gradients: f32 [n_slots, channels, states]. */
 typedef struct {
   sparsl_seqs seqs;

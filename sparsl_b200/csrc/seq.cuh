@@ -249,7 +249,7 @@ struct SscanArgs {
   // Row strides in bytes (the launch fills them in): a row's address is one 32 x 32 -> 64 bit product.
   uint32_t x_row, dt_row, z_row, y_row, dy_row, dx_row, ddt_row, dz_row;
 };
-constexpr uint64_t kMostStride = (1u << 29) - 1;  // elements: 4-byte rows of it still count in 31 bits
+constexpr uint64_t kMostStride = (1u << 29) - 1;  // elements from token to token: 4-byte rows of it still count in 31 bits
 constexpr uint32_t kMaxStates = 64;
 size_t sscan_bytes(uint64_t tokens, uint64_t channels, uint32_t states, uint64_t n_seq, uint32_t groups);
 size_t sscan_backward_bytes(uint64_t tokens, uint64_t channels, uint32_t states, uint64_t n_seq, uint32_t groups);

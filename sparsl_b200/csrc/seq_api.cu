@@ -69,6 +69,7 @@ bool inside_allocation(const void* p, uint64_t bytes, int ordinal) {
 
 constexpr uint64_t kMostRows = 0x7fffffffull;  // seq_ptr's type
 constexpr uint64_t kMostBytes = 1ull << 62;
+constexpr uint64_t kMostGroup = 1ull << 36;  // elements from group to group: 2^24 of them fit 64 bits
 
 // A device array of a call: `rows` rows of `width` elements of `size` bytes,
 // `stride` elements apart.
@@ -119,10 +120,6 @@ struct Call {
       fail(SPARSL_ERR_LENGTH, "row stride", std::string(name) + ": rows overlap (the stride is below the row's length)");
       return;
     }
-    if (stride > kMostStride) {
-      fail(SPARSL_ERR_LENGTH, "row stride", std::string(name) + ": the row stride is too large");
-      return;
-    }
     const Array a{name, p, rows, width, stride, size, out};
     if (a.bytes() >= kMostBytes) {
       fail(SPARSL_ERR_LENGTH, "array size", std::string(name) + ": the array is too large");
@@ -143,6 +140,11 @@ struct Call {
   }
   void rows(const char* name, const sparsl_rows& r, uint64_t n, uint64_t width, uint64_t size, bool out, bool optional = false) {
     add(name, r.p, n, width, r.stride, size, out, optional);
+  }
+  // The same for the scan, whose kernels count a row's bytes in 31 bits.
+  void scan_rows(const char* name, const sparsl_rows& r, uint64_t n, uint64_t width, uint64_t size, bool out, bool optional = false) {
+    if ((r.p || !optional) && n > 1) want(r.stride <= kMostStride, SPARSL_ERR_LENGTH, "row stride", "a row stride is above 2^29 - 1 elements");
+    rows(name, r, n, width, size, out, optional);
   }
   void flat(const char* name, const void* p, uint64_t n, uint64_t size, bool out, bool optional = false) {
     add(name, p, n ? 1 : 0, n, n, size, out, optional);
@@ -317,12 +319,12 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
     const uint64_t row = ch * n;
     const auto bc = [&](const char* name, const sparsl_rows& r, uint64_t group, bool out) {
       k.want(g == 1 || group >= n, SPARSL_ERR_LENGTH, "group stride", "the runs of b or c overlap");
-      k.want(group <= kMostStride, SPARSL_ERR_LENGTH, "group stride", "the group stride is too large");
+      k.want(group <= kMostGroup, SPARSL_ERR_LENGTH, "group stride", "the group stride is too large");
       k.rows(name, r, t, (g == 1 ? 0 : (g - 1) * group) + n, e, out);
     };
-    k.rows("x", p->x, t, ch, e, false);
-    k.rows("dt", p->dt, t, ch, e, false);
-    k.rows("z", p->z, t, ch, e, false, true);
+    k.scan_rows("x", p->x, t, ch, e, false);
+    k.scan_rows("dt", p->dt, t, ch, e, false);
+    k.scan_rows("z", p->z, t, ch, e, false, true);
     bc("b", p->b, p->b_group, false);
     bc("c", p->c, p->c_group, false);
     k.flat("a", p->a, row, 4, false);
@@ -359,10 +361,10 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
     if (!step && (back || p->checkpoints))
       k.scratch("checkpoints", p->checkpoints, p->checkpoint_bytes, sscan_mark_bytes(t, ch, p->states), !back);
     if (back) {
-      k.rows("dy", p->dy, t, ch, e, false);
-      k.rows("dx", p->dx, t, ch, e, true);
-      k.rows("ddt", p->ddt, t, ch, e, true);
-      if (p->z.p) k.rows("dz", p->dz, t, ch, e, true);
+      k.scan_rows("dy", p->dy, t, ch, e, false);
+      k.scan_rows("dx", p->dx, t, ch, e, true);
+      k.scan_rows("ddt", p->ddt, t, ch, e, true);
+      if (p->z.p) k.scan_rows("dz", p->dz, t, ch, e, true);
       bc("db", p->db, p->db_group, true);
       bc("dc", p->dc, p->dc_group, true);
       k.flat("da", p->da, row, 4, true);
@@ -397,7 +399,7 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
       a.dfinal = p->dfinal_state;
       return k.rc != SPARSL_OK ? k.rc : k.done(launch_sscan_backward(a, stream_of(d, stream)));
     }
-    k.rows("y", p->y, t, ch, e, true);
+    k.scan_rows("y", p->y, t, ch, e, true);
     k.add("final_state", p->final_state, p->seqs.n_slots, row, row, 4, true, !step);
     if (!step) k.scratch("workspace", p->workspace, p->workspace_bytes, sscan_bytes(t, ch, p->states, p->seqs.n_seq, p->groups));
     k.apart(step ? nullptr : p->state);

@@ -321,6 +321,49 @@ def test_scan_far_states(cuda_device):
     R.check(yt, want["y"][0][:1], want["y"][1][:1], k, "step")
 
 
+def test_kept_states_and_workspaces_past_half_a_gigabyte(cuda_device):
+    """129 equal sequences whose kept states and workspace pass 2^29 bytes give what one gives, bit for bit."""
+    dev, st = cuda_device, _stream()
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("the arrays do not fit this GPU")
+    n, length, ch, ns, dtype = 129, 64, 2048, 64, torch.bfloat16
+    one = Scan([length], ch, ns, dtype=dtype, ragged=False)
+    names = ("x", "dt", "z", "b", "c", "dy")
+    rows = {k: getattr(one, k).repeat(n, *([1] * (getattr(one, k).dim() - 1))) for k in names}
+    t = n * length
+    assert dev.selective_scan_checkpoints(t, ch, ns) >= 1 << 29
+    assert dev.selective_scan_backward_workspace(t, ch, ns, n) >= 1 << 29
+
+    def both(x, dt, z, b, c, dy, n):
+        t = x.shape[0]
+        y, dx, ddt, dz = (torch.zeros_like(x) for _ in range(4))
+        db, dc, da, dd, dbias = (torch.zeros(k.shape, dtype=k.dtype, device="cuda") for k in (b, c, one.a, one.d, one.bias))
+        marks = _room(dev.selective_scan_checkpoints(t, ch, ns))
+        room = _room(max(dev.selective_scan_workspace(t, ch, ns, n), dev.selective_scan_backward_workspace(t, ch, ns, n)))
+        dev.selective_scan_device(x, dt, one.a, b, c, y, room, d=one.d, z=z, dt_bias=one.bias, softplus=True, n_seq=n,
+                                  checkpoints=marks, stream=st)
+        dev.selective_scan_backward_device(dy, x, dt, one.a, b, c, marks, dx, ddt, da, db, dc, room, d=one.d, dd=dd, z=z, dz=dz,
+                                           dt_bias=one.bias, ddt_bias=dbias, softplus=True, n_seq=n, stream=st)
+        return (y, dx, ddt, dz, db, dc), (da, dd, dbias)
+
+    small, small_sums = both(*(getattr(one, k).contiguous() for k in names), 1)
+    large, sums = both(*(rows[k] for k in names), n)
+    for p, q in zip(small, large):
+        assert torch.equal(q.unflatten(0, (n, length)), p.expand(n, *p.shape))
+    for p, q in zip(small_sums, sums):  # n equal terms, each addition rounded once
+        assert ((q.double() - n * p.double()).abs() <= n * 2.0 ** -24 * n * p.double().abs()).all()
+
+
+def test_rows_of_the_scan_lie_within_their_reach(cuda_device):
+    """The scan counts a row's bytes in 31 bits: longer strides are refused."""
+    s = Scan([2], 4, 4)
+    far = torch.empty((1 << 29) + 8, dtype=torch.bfloat16, device="cuda").as_strided((2, 4), (1 << 29, 1))
+    args = [v.to(torch.bfloat16) for v in (s.x, s.dt)]
+    bc = [v.to(torch.bfloat16).contiguous() for v in (s.b, s.c)]
+    assert "stride" in _refused("Length", cuda_device.selective_scan_device, far, args[1], s.a, *bc, torch.zeros_like(args[0]), None,
+                                stream=_stream())
+
+
 # ---- the causal convolution ----------------------------------------------------------------------
 
 
@@ -577,6 +620,16 @@ def test_norm_far_rows(cuda_device):
     cuda_device.layer_norm_device(x, y, stream=_stream())
     cuda_device.layer_norm_device(x.contiguous(), z, stream=_stream())
     assert torch.equal(y, z)
+
+
+def test_norm_of_more_than_half_a_billion_rows(cuda_device):
+    rows = (1 << 29) + 8
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("the rows do not fit this GPU")
+    x = torch.randn(rows, 1, dtype=torch.bfloat16, device="cuda")
+    y, mean = torch.ones_like(x), torch.zeros(rows, device="cuda")
+    cuda_device.layer_norm_device(x, y, mean=mean, stream=_stream())
+    assert (y == 0).all() and torch.equal(mean, x[:, 0].float())
 
 
 # ---- streams, graphs, refusals, and the operators together ----------------------------------------------
