@@ -78,6 +78,7 @@ struct Array {
   const void* p;
   uint64_t rows, width, stride, size;
   bool out;
+  bool state = false;  // a call's state or final state
   uint64_t bytes() const {
     if (!rows || !width) return 0;
     const unsigned __int128 b = ((unsigned __int128)(rows - 1) * stride + width) * size;
@@ -146,6 +147,12 @@ struct Call {
     if ((r.p || !optional) && n > 1) want(r.stride <= kMostStride, SPARSL_ERR_LENGTH, "row stride", "a row stride is above 2^29 - 1 elements");
     rows(name, r, n, width, size, out, optional);
   }
+  // The state a call starts from, or the one it leaves.
+  void states(const char* name, const void* p, uint64_t n, uint64_t row, uint64_t size, bool out, bool optional) {
+    const int before = count;
+    add(name, p, n, row, row, size, out, optional);
+    if (count > before) arrays[before].state = true;
+  }
   void flat(const char* name, const void* p, uint64_t n, uint64_t size, bool out, bool optional = false) {
     add(name, p, n ? 1 : 0, n, n, size, out, optional);
   }
@@ -163,12 +170,13 @@ struct Call {
     }
     add(name, p, 1, need, need, 1, out);
   }
-  // Outputs apart from everything else; `in_place`: the state pair may be one array.
-  void apart(const void* in_place = nullptr) {
+  // Outputs apart from everything else.  A state and its final state (`state` and
+  // `final_state`, arrays of one size) may be the same array.
+  void apart() {
     for (int i = 0; i < count && rc == SPARSL_OK; ++i)
       for (int j = i + 1; j < count; ++j) {
         if (!arrays[i].out && !arrays[j].out) continue;
-        if (in_place && arrays[i].p == in_place && arrays[j].p == in_place && arrays[i].bytes() == arrays[j].bytes()) continue;
+        if (arrays[i].state && arrays[j].state && arrays[i].p == arrays[j].p) continue;
         if (overlap(arrays[i], arrays[j])) {
           fail(SPARSL_ERR_INVALID, "overlap", std::string(arrays[i].name) + " and " + arrays[j].name + " overlap");
           return;
@@ -258,7 +266,7 @@ int conv(sparsl_dev* d, const sparsl_conv_args* p, void* stream, const char* op,
     k.rows("x", p->x, t, ch, e, false);
     k.flat("weight", p->weight, ch * w, pe, false);
     k.flat("bias", p->bias, ch, pe, false, true);
-    if (!step) k.add("state", p->state, p->seqs.n_slots, row, row, e, false, true);
+    if (!step) k.states("state", p->state, p->seqs.n_slots, row, e, false, true);
     a.type = p->dtype;
     a.channels = p->channels;
     a.width = p->width;
@@ -290,8 +298,8 @@ int conv(sparsl_dev* d, const sparsl_conv_args* p, void* stream, const char* op,
       return k.rc != SPARSL_OK ? k.rc : k.done(launch_conv_backward(a, stream_of(d, stream)));
     }
     k.rows("y", p->y, t, ch, e, true);
-    k.add("final_state", p->final_state, p->seqs.n_slots, row, row, e, true, !step);
-    k.apart(step ? nullptr : p->state);
+    k.states("final_state", p->final_state, p->seqs.n_slots, row, e, true, !step);
+    k.apart();
     a.y = p->y.p;
     a.y_stride = p->y.stride;
     a.final_state = p->final_state;
@@ -330,7 +338,7 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
     k.flat("a", p->a, row, 4, false);
     k.flat("d", p->d, ch, 4, false, true);
     k.flat("dt_bias", p->dt_bias, ch, 4, false, true);
-    if (!step) k.add("state", p->state, p->seqs.n_slots, row, row, 4, false, true);
+    if (!step) k.states("state", p->state, p->seqs.n_slots, row, 4, false, true);
     a.type = p->dtype;
     a.channels = p->channels;
     a.states = p->states;
@@ -400,9 +408,9 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
       return k.rc != SPARSL_OK ? k.rc : k.done(launch_sscan_backward(a, stream_of(d, stream)));
     }
     k.scan_rows("y", p->y, t, ch, e, true);
-    k.add("final_state", p->final_state, p->seqs.n_slots, row, row, 4, true, !step);
+    k.states("final_state", p->final_state, p->seqs.n_slots, row, 4, true, !step);
     if (!step) k.scratch("workspace", p->workspace, p->workspace_bytes, sscan_bytes(t, ch, p->states, p->seqs.n_seq, p->groups));
-    k.apart(step ? nullptr : p->state);
+    k.apart();
     a.y = p->y.p;
     a.y_stride = p->y.stride;
     a.y_row = bytes(p->y);

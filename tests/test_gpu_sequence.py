@@ -819,6 +819,25 @@ def test_refusals(cuda_device):
     torch.cuda.synchronize()
 
 
+def test_only_the_final_state_may_be_the_state(cuda_device):
+    """Outputs that are the state's own bytes in another role are refused, equal sizes or not."""
+    dev, st = cuda_device, _stream()
+    ch, width = 16, 4
+    v = Conv([3, 3], ch, width)  # 6 tokens: as many values as two states
+    state = torch.zeros(2, width - 1, ch, device="cuda")
+    y = state.view(6, ch)
+    assert "overlap" in _refused("Backend", dev.causal_conv_device, v.x, v.w, y, seq_ptr=v.ptr, state=state, stream=st)
+    _refused("Backend", dev.causal_conv_device, v.x, v.w, y, seq_ptr=v.ptr, final_state=state, stream=st)
+    _refused("Backend", dev.causal_conv_device, v.x, v.w, y, seq_ptr=v.ptr, state=state, final_state=state, stream=st)
+    s = Scan([4, 4], ch, 4)  # 8 tokens: as many values as two states
+    state = torch.zeros(2, ch, 4, device="cuda")
+    args = (s.x, s.dt, s.a, s.b, s.c)
+    _refused("Backend", dev.selective_scan_device, *args, state.view(8, ch), seq_ptr=s.ptr, state=state, stream=st)
+    _refused("Backend", dev.selective_scan_step_device, s.x[:2], s.dt[:2], s.a, s.b[:2], s.c[:2], state.view(8, ch)[:2], state, stream=st)
+    torch.cuda.synchronize()
+    assert (state == 0).all()
+
+
 def test_a_layer_of_them(cuda_device):
     """norm -> projection -> convolution -> projection -> scan, its gradients against autograd in 64 bits, and a token more
     through the kept states against the prompt that holds it."""
