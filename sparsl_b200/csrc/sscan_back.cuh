@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
         float v = 0.f;
 #pragma unroll
         for (int q = 0; q < kWarps; ++q) v += sh.red[out][q][which][k][n];
-        to[k * part_row + which * N + n] = v;
+        to[(uint64_t)k * part_row + which * N + n] = v;
       }
       out ^= 1;  // the next block of tokens writes the other one while this is read
     }

@@ -364,6 +364,30 @@ def test_rows_of_the_scan_lie_within_their_reach(cuda_device):
                                 stream=_stream())
 
 
+def test_scan_gradients_of_very_many_groups(cuda_device):
+    """The partial sums of eight tokens' B and C pass 2^32 values: each group gives what one alone gives, bit for bit."""
+    dev, st = cuda_device, _stream()
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("the groups do not fit this GPU")
+    n, ns, t = 4_800_000, 64, 8
+    one = Scan([t], 1, ns, dtype=torch.bfloat16, gate=False, skip=False, bias=False, softplus=False, ragged=False)
+
+    def grads(n):
+        x, dt, dy = (v.expand(t, n).contiguous() for v in (one.x, one.dt, one.dy))
+        a = one.a.expand(n, ns).contiguous()
+        b, c = (v.expand(t, n, ns).contiguous() for v in (one.b, one.c))
+        y, dx, ddt, da, db, dc = (torch.zeros_like(v) for v in (x, x, x, a, b, c))
+        marks = _room(dev.selective_scan_checkpoints(t, n, ns))
+        room = _room(dev.selective_scan_backward_workspace(t, n, ns, 1, n))
+        dev.selective_scan_device(x, dt, a, b, c, y, None, checkpoints=marks, stream=st)
+        dev.selective_scan_backward_device(dy, x, dt, a, b, c, marks, dx, ddt, da, db, dc, room, stream=st)
+        return y, dx, ddt, da[None], db, dc
+
+    alone = grads(1)
+    for p, q in zip(alone, grads(n)):
+        assert (q == p.expand_as(q)).all()
+
+
 # ---- the causal convolution ----------------------------------------------------------------------
 
 
