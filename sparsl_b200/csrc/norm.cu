@@ -401,17 +401,20 @@ cudaError_t go(const NormArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+// `most` is what the kernel may ever take: the setting is the kernel's, not the
+// launch's, and another thread's call must not find it lowered.
 template <class K>
-cudaError_t allow(K kernel, int bytes) {
-  return bytes > 40 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;
+cudaError_t allow(K kernel, int most) {
+  return most > 40 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) : cudaSuccess;
 }
 
 template <class T, int V, int B, int VALUES>
 cudaError_t go_rows(const NormArgs& a, cudaStream_t s) {
   constexpr int kSide = 256 / B, kStages = 2;
-  const int bytes = (int)((a.channels + 3) / 4 * 4 * 8) + 256 * RowsAhead<T, V, B, VALUES / V, 1, kStages>::kBytes;
+  constexpr int kAhead = 256 * RowsAhead<T, V, B, VALUES / V, 1, kStages>::kBytes;
+  const int bytes = (int)((a.channels + 3) / 4 * 4 * 8) + kAhead;
   const auto kernel = norm_rows_kernel<T, V, B, VALUES / V, kStages>;
-  const cudaError_t e = allow(kernel, bytes);
+  const cudaError_t e = allow(kernel, B * VALUES * 8 + kAhead);
   if (e != cudaSuccess) return e;
   const uint64_t blocks = (a.rows + kSide - 1) / kSide, fit = 220 * 1024 / bytes, regs = VALUES >= 64 ? 2 : VALUES >= 24 ? 3 : 5;
   const uint64_t most = (uint64_t)kSms * (fit < regs ? (fit ? fit : 1) : regs);

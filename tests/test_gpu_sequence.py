@@ -386,6 +386,8 @@ def test_scan_gradients_of_very_many_groups(cuda_device):
     alone = grads(1)
     for p, q in zip(alone, grads(n)):
         assert (q == p.expand_as(q)).all()
+    del q
+    torch.cuda.empty_cache()  # 45 GB
 
 
 # ---- the causal convolution ----------------------------------------------------------------------
@@ -654,6 +656,8 @@ def test_norm_of_more_than_half_a_billion_rows(cuda_device):
     y, mean = torch.ones_like(x), torch.zeros(rows, device="cuda")
     cuda_device.layer_norm_device(x, y, mean=mean, stream=_stream())
     assert (y == 0).all() and torch.equal(mean, x[:, 0].float())
+    del x, y, mean
+    torch.cuda.empty_cache()
 
 
 # ---- streams, graphs, refusals, and the operators together ----------------------------------------------
@@ -742,6 +746,37 @@ def test_two_threads_at_once(cuda_device):
             failed.append(e)
 
     threads = [threading.Thread(target=work, args=a) for a in zip(sets, marks, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
+def test_norms_of_two_widths_from_two_threads(cuda_device):
+    """Widths that share a kernel but not its shared memory's size, called at once."""
+    import threading
+
+    sets = []
+    for ch in (2056, 4096):
+        x = torch.randn(2400, ch, device="cuda")
+        y = torch.zeros_like(x)
+        cuda_device.layer_norm_device(x, y, stream=_stream())
+        sets.append((x, y))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(x, want):
+        try:
+            side, y = torch.cuda.Stream(), torch.zeros_like(x)
+            for _ in range(3000):
+                cuda_device.layer_norm_device(x, y, stream=side)
+            side.synchronize()
+            assert torch.equal(y, want)
+        except Exception as e:  # noqa: BLE001 (reported by the main thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in sets]
     for t in threads:
         t.start()
     for t in threads:
