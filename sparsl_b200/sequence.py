@@ -6,7 +6,8 @@ Arrays are device arrays of the device's GPU: torch tensors, or objects with
 ``data_ptr()``, ``shape``, ``stride()`` and ``dtype``.  Token arrays are
 [tokens, channels] with the channels next to each other; rows may be strided, so
 column ranges of a wider array serve as they are.  Every call only enqueues its
-work: on ``stream`` (a cudaStream_t or a torch stream), or on the device's own.
+work: on ``stream`` (a cudaStream_t, 0 the legacy default stream, or a torch
+stream), or, with None, on the device's own, which does not wait for torch's.
 Outputs are the caller's arrays; an output must not overlap an input.
 """
 from __future__ import annotations
@@ -139,11 +140,12 @@ def _scratch(t):
 
 
 def _stream(stream):
-    """A cudaStream_t for the C ABI.  A torch stream's handle, where 0 means CUDA's
-    legacy default stream; None is the device's own stream."""
-    if stream is None or isinstance(stream, int):
-        return stream
-    return stream.cuda_stream or 1  # cudaStreamLegacy
+    """A cudaStream_t for the C ABI: a stream's handle or a torch stream's, where 0 is
+    CUDA's legacy default stream (NULL would be the device's own there); None is the
+    device's own stream."""
+    if stream is None:
+        return None
+    return (stream if isinstance(stream, int) else stream.cuda_stream) or 1  # cudaStreamLegacy
 
 
 # The argument blocks of include/sparsl_cuda.h, packed in one go (filling

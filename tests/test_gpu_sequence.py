@@ -723,6 +723,22 @@ def test_other_streams(cuda_device):
     assert torch.equal(y1, y2) and torch.equal(y1, y3)
 
 
+def test_the_default_streams_handle_is_that_stream(cuda_device):
+    """A call on the handle of torch's default stream, 0, follows the work that makes its inputs there."""
+    x, y = torch.zeros(4096, 4096, device="cuda"), torch.zeros(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for k in range(1, 4):
+        for _ in range(40):  # some milliseconds of work in front of the input
+            x.add_(1.0)
+        x.copy_(torch.arange(4096, device="cuda", dtype=torch.float32).expand(4096, 4096) * k)
+        cuda_device.layer_norm_device(x, y, eps=0.0, stream=torch.cuda.default_stream().cuda_stream)
+        want = y.clone()
+        torch.cuda.synchronize()
+        cuda_device.layer_norm_device(x, y, eps=0.0)
+        cuda_device.wait()
+        assert torch.equal(want, y) and torch.isfinite(y).all()
+
+
 def test_two_threads_at_once(cuda_device):
     """Calls from two threads, each on its own stream with its own arrays, give what they give alone."""
     import threading

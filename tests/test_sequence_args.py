@@ -152,3 +152,10 @@ def test_workspace_sizes():
     assert D.selective_scan_checkpoints(17, 10, 16) == 3 * 10 * 16 * 4
     assert D.selective_scan_backward_workspace(100, 64, 16, 1, 3) == 0  # 64 channels are no 3 groups: nothing to size
     assert D.layer_norm_backward_workspace(10, 100) == 10 * 2 * 100 * 4
+
+
+def test_a_handle_is_the_stream_it_comes_from():
+    """0, the handle of torch's default stream, is that stream, not the device's own."""
+    from sparsl_b200.sequence import _stream
+
+    assert _stream(0) == 1 == _stream(types.SimpleNamespace(cuda_stream=0)) and _stream(1) == 1 and _stream(None) is None
