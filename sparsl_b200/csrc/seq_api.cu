@@ -79,6 +79,8 @@ struct Array {
   uint64_t rows, width, stride, size;
   bool out;
   bool state = false;  // a call's state or final state
+  // A row of `width` elements may be runs of `run` ones, `group` apart (0: one run).
+  uint64_t group = 0, run = 0;
   uint64_t bytes() const {
     if (!rows || !width) return 0;
     const unsigned __int128 b = ((unsigned __int128)(rows - 1) * stride + width) * size;
@@ -86,17 +88,31 @@ struct Array {
   }
 };
 
+// Whether the rows of two arrays in runs, b's `off` bytes behind a's, may share an
+// element: by where in a group their runs lie.
+bool runs_meet(const Array& a, const Array& b, uint64_t off) {
+  const uint64_t group = a.group * a.size;
+  if (!group || group != b.group * b.size) return true;
+  const uint64_t at = off % group;
+  return at < a.run * a.size || group - at < b.run * b.size;
+}
+
 // Whether two arrays share an element.  Rows of one stride (column ranges of
-// one wide array) may interleave.
+// one wide array) may interleave, and so may the runs of their rows.
 bool overlap(const Array& a, const Array& b) {
   const uint64_t na = a.bytes(), nb = b.bytes();
   if (!na || !nb) return false;
   const uint64_t pa = reinterpret_cast<uint64_t>(a.p), pb = reinterpret_cast<uint64_t>(b.p);
   if (pa + na <= pb || pb + nb <= pa) return false;
+  if (a.rows < 2 && b.rows < 2) return pb >= pa ? runs_meet(a, b, pb - pa) : runs_meet(b, a, pa - pb);
   const uint64_t sa = a.stride * a.size, sb = b.stride * b.size;
   if (sa != sb || a.rows < 2 || b.rows < 2 || !sa) return true;
+  const uint64_t wa = a.width * a.size, wb = b.width * b.size;
   const uint64_t off = pb >= pa ? (pb - pa) % sa : (sa - (pa - pb) % sa) % sa;  // b's columns behind a's
-  return off < a.width * a.size || sa - off < b.width * b.size;
+  if (off >= wa && sa - off >= wb) return false;
+  if (off + wb <= sa) return runs_meet(a, b, off);  // b's row ends before a's next one begins
+  if (wa <= off) return runs_meet(b, a, sa - off);  // a's row ends before b's next one begins
+  return true;
 }
 
 struct Call {
@@ -146,6 +162,15 @@ struct Call {
   void scan_rows(const char* name, const sparsl_rows& r, uint64_t n, uint64_t width, uint64_t size, bool out, bool optional = false) {
     if ((r.p || !optional) && n > 1) want(r.stride <= kMostStride, SPARSL_ERR_LENGTH, "row stride", "a row stride is above 2^29 - 1 elements");
     rows(name, r, n, width, size, out, optional);
+  }
+  // Rows of `groups` runs of `run` elements, `group` apart.
+  void runs(const char* name, const sparsl_rows& r, uint64_t n, uint64_t groups, uint64_t group, uint64_t run, uint64_t size, bool out) {
+    const int before = count;
+    rows(name, r, n, (groups == 1 ? 0 : (groups - 1) * group) + run, size, out);
+    if (count > before && groups > 1) {
+      arrays[before].group = group;
+      arrays[before].run = run;
+    }
   }
   // The state a call starts from, or the one it leaves.
   void states(const char* name, const void* p, uint64_t n, uint64_t row, uint64_t size, bool out, bool optional) {
@@ -328,7 +353,7 @@ int scan(sparsl_dev* d, const sparsl_scan_args* p, void* stream, const char* op,
     const auto bc = [&](const char* name, const sparsl_rows& r, uint64_t group, bool out) {
       k.want(g == 1 || group >= n, SPARSL_ERR_LENGTH, "group stride", "the runs of b or c overlap");
       k.want(group <= kMostGroup, SPARSL_ERR_LENGTH, "group stride", "the group stride is too large");
-      k.rows(name, r, t, (g == 1 ? 0 : (g - 1) * group) + n, e, out);
+      k.runs(name, r, t, g, group, n, e, out);
     };
     k.scan_rows("x", p->x, t, ch, e, false);
     k.scan_rows("dt", p->dt, t, ch, e, false);

@@ -913,6 +913,43 @@ def test_only_the_final_state_may_be_the_state(cuda_device):
     assert (state == 0).all()
 
 
+def test_gradients_of_interleaved_runs(cuda_device):
+    """db and dc may interleave group by group, as b and c may: [tokens, groups, 2, states]; runs that meet are refused."""
+    dev = cuda_device
+    for tail in (0, 5):  # rows that hold whole groups only, and some columns more
+        s = Scan([40, 3], 24, 8, groups=3, dtype=torch.bfloat16)
+        marks = s.marks(dev)
+        s.forward(dev, marks=marks)
+        want = s.backward(dev, marks)
+        wide = torch.full((43, 3 * 2 * 8 + tail), 7.0, dtype=torch.bfloat16, device="cuda")
+        runs = wide[:, :48].unflatten(1, (3, 2, 8))
+        out = {k: torch.zeros_like(want[k]) for k in ("dx", "ddt", "dz", "da", "dd", "ddt_bias")}
+        room = _room(dev.selective_scan_backward_workspace(43, 24, 8, 2, 3))
+
+        def run(db, dc):
+            dev.selective_scan_backward_device(s.dy, s.x, s.dt, s.a, s.b, s.c, marks, out["dx"], out["ddt"], out["da"], db, dc, room,
+                                               d=s.d, dd=out["dd"], z=s.z, dz=out["dz"], dt_bias=s.bias, ddt_bias=out["ddt_bias"],
+                                               softplus=True, seq_ptr=s.ptr, stream=_stream())
+
+        run(runs[:, :, 0], runs[:, :, 1])
+        assert torch.equal(runs[:, :, 0], want["db"]) and torch.equal(runs[:, :, 1], want["dc"])
+        run(runs[:, :, 1], runs[:, :, 0])
+        assert torch.equal(runs[:, :, 1], want["db"]) and torch.equal(runs[:, :, 0], want["dc"])
+        assert (wide[:, 48:] == 7).all()
+        meet = wide[:, 1:1 + 40].unflatten(1, (5, 8))[:, ::2] if tail else wide[:, :40].unflatten(1, (5, 8))[:, ::2]
+        _refused("Backend", run, runs[:, :, 0], meet)
+    one = torch.zeros(1, 48, dtype=torch.bfloat16, device="cuda").unflatten(1, (3, 2, 8))  # a single token
+    s = Scan([1], 24, 8, groups=3, dtype=torch.bfloat16)
+    marks = s.marks(dev)
+    s.forward(dev, marks=marks)
+    want = s.backward(dev, marks)
+    dx, ddt, dz, da = (torch.zeros_like(v) for v in (s.x, s.x, s.x, s.a))
+    room = _room(dev.selective_scan_backward_workspace(1, 24, 8, 1, 3))
+    dev.selective_scan_backward_device(s.dy, s.x, s.dt, s.a, s.b, s.c, marks, dx, ddt, da, one[:, :, 0], one[:, :, 1], room, d=s.d, z=s.z,
+                                       dz=dz, dt_bias=s.bias, softplus=True, seq_ptr=s.ptr, stream=_stream())
+    assert torch.equal(one[:, :, 0], want["db"]) and torch.equal(one[:, :, 1], want["dc"])
+
+
 def test_a_layer_of_them(cuda_device):
     """norm -> projection -> convolution -> projection -> scan, its gradients against autograd in 64 bits, and a token more
     through the kept states against the prompt that holds it."""
