@@ -136,6 +136,16 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_chunk_kernel(Ss
   }
 }
 
+// A state behind a chunk: `carry` in front of it decayed by 2^x, and what the chunk
+// itself hands on.  2^x may leave f32's range where no token's decay and no state
+// does: it is then applied by halves, and never to a state of zero.
+__device__ __forceinline__ float behind_chunk(float x, float carry, float own) {
+  if (fabsf(x) < 120.0f) return __fmaf_rn(ex2(x), carry, own);
+  if (carry == 0.0f) return own;
+  const float half = ex2(0.5f * x);
+  return __fmaf_rn(half, half * carry, own);
+}
+
 // What each chunk starts from, in place of what it hands on: ascending for the
 // states, descending (BACK) for their gradients.
 template <bool BACK>
@@ -164,7 +174,7 @@ __global__ void __launch_bounds__(128) sscan_fold_kernel(const float* a, ScanWor
       if (k + u < chunks) {
         const uint64_t j = BACK ? chunks - 1 - (k + u) : k + u;
         w.state[j * cells + i] = carry;
-        carry = cut[u] == 2 ? 0.f : cut[u] == 1 ? v[u] : __fmaf_rn(ex2(s[u] * a2), carry, v[u]);
+        carry = cut[u] == 2 ? 0.f : cut[u] == 1 ? v[u] : behind_chunk(s[u] * a2, carry, v[u]);
       }
   }
 }

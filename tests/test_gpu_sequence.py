@@ -301,6 +301,31 @@ def test_scan_infinite_and_nan_stay_in_their_sequence(cuda_device):
     assert torch.equal(y[50:55], clean[50:55])
 
 
+@pytest.mark.parametrize("start,rate", [(1e-30, 1.45), (0.0, 2.0), (1e30, -1.45)])
+def test_states_across_chunks_that_grow_or_fade_past_a_float(cuda_device, start, rate):
+    """A chunk's whole decay may leave f32's range where no state does: exp(+-93) of a state of 1e-+30, exp(128) of none."""
+    t, ch, ns, chunk = 192, 8, 4, 64
+    x = torch.zeros(t, ch, device="cuda")
+    x[2 * chunk:] = 1
+    dt = torch.zeros(t, ch, device="cuda")
+    dt[chunk:2 * chunk] = 1
+    dt[2 * chunk:] = 2.0 ** -10
+    a = torch.full((ch, ns), rate, device="cuda")
+    b, c = torch.full((t, ns), 0.0 if start else 1.0, device="cuda"), torch.ones(t, ns, device="cuda")
+    state = torch.full((1, ch, ns), start, device="cuda")
+    y, final = torch.zeros_like(x), torch.zeros_like(state)
+    assert cuda_device.selective_scan_workspace(t, ch, ns, 1, 1) > 0  # chunks
+    room = _room(cuda_device.selective_scan_workspace(t, ch, ns, 1, 1))
+    ptr = torch.tensor([0, t], dtype=torch.int32).cuda()
+    cuda_device.selective_scan_device(x, dt, a, b, c, y, room, seq_ptr=ptr, state=state, final_state=final, stream=_stream())
+    leaf = [_up(v) for v in (x, dt, a, b[:, None], c[:, None])]
+    want, last = R.scan(*leaf, None, None, None, False, [t], _up(state))
+    most, most_last = R.scan(*leaf, None, None, None, False, [t], _up(state), magnitude=True)
+    k = R.scan_bound(_up(dt), _up(a), None, False, [t], t, ch)
+    R.check(y, want, most, k, "y")
+    R.check(final, last, most_last, k, "final")
+
+
 def test_scan_far_states(cuda_device):
     """A pool whose rows lie past 2^32 bytes and 2^31 values."""
     ch, ns, rows = 2048, 16, 70000
