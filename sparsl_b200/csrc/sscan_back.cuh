@@ -240,7 +240,8 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
   const uint64_t row = ((uint64_t)chunk * a.channels + me.c) * N;
   if (p.carry && me.valid) load_pairs<NS, FULL>(w.scan.state + row, me.n0, N, r);
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
-  const float dskip = a.d ? a.d[me.c] : 0.f;
+  const bool skip = a.d != nullptr;  // without it no term: 0 times an infinite value would be NaN
+  const float dskip = skip ? a.d[me.c] : 0.f;
   float dd = 0.f, dbias = 0.f;
   const auto state_row = [&](int64_t seq) {
     const int64_t slot = a.seq.slot(seq);
@@ -384,7 +385,8 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
           if (GATE) {
             o[q] = sum2(oo);
             if (q == LP - 1) {
-              const float pre = __fmaf_rn(dskip, xv[j], scatter_sum<LP>(o, part));
+              float pre = scatter_sum<LP>(o, part);
+              if (skip) pre = __fmaf_rn(dskip, xv[j], pre);
               result[2][j * LP + part][col] = from_f32<T>(gg[j] * pre);
             }
           }
@@ -434,7 +436,8 @@ __global__ void __launch_bounds__(kScanThreads, resident(NS)) sscan_back_kernel(
             const float ds = (live >> (j * LP + part) & 1) ? __fmaf_rn(gas, 1.0f / kLog2e, xv[j] * gbs) * slope[j] : 0.f;
             dd_block = __fmaf_rn(g[j], xv[j], dd_block);
             dbias_block += ds;
-            result[0][j * LP + part][col] = from_f32<T>(__fmaf_rn(dskip, g[j], s[j] * gbs));
+            const float through_b = s[j] * gbs;
+            result[0][j * LP + part][col] = from_f32<T>(skip ? __fmaf_rn(dskip, g[j], through_b) : through_b);
             result[1][j * LP + part][col] = from_f32<T>(ds);
           }
           if ((EDGES || k == 0) && (start >> k & 1)) {

@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArg
   const uint64_t row = ((uint64_t)chunk * a.channels + me.c) * N;
   if (p.carry) load_pairs<NS, FULL>(w.state + row, me.n0, N, h);
   const float bias = a.dt_bias ? a.dt_bias[me.c] : 0.f;
-  const float dskip = a.d ? a.d[me.c] : 0.f;
+  const bool skip = a.d != nullptr;  // without it no term: 0 times an infinite x would be NaN
+  const float dskip = skip ? a.d[me.c] : 0.f;
 
   const auto begin_state = [&](int64_t seq) {
     zero_pairs(h);
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArg
       store_pairs<NS, FULL>(a.marks + ((uint64_t)(t / kMarkEvery) * a.channels + me.c) * N, me.n0, N, h);
   };
   const auto finish = [&](float o, float xv, float zv) {
-    o = __fmaf_rn(dskip, xv, o);
+    if (skip) o = __fmaf_rn(dskip, xv, o);
     if (GATE) o *= zv * sigmoid(zv);
     return from_f32<T>(o);
   };
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(kScanThreads, kResident) sscan_step_many_kerne
     decay<NS>(step, a2, e);
     advance<NS, FULL>(e, step * xv[u], &bc[u][0][me.n0], me.n0, N, h[u]);
     float o = sum_lanes<LP>(dot<NS>(&bc[u][1][me.n0], h[u]));
-    o = __fmaf_rn(dskip, xv[u], o);
+    if (a.d) o = __fmaf_rn(dskip, xv[u], o);
     if (a.z) o *= zv[u] * sigmoid(zv[u]);
     if (!me.valid) continue;
     store_rows<NS, FULL>(a.final_state + at[u], me.n0, N, h[u]);

@@ -326,6 +326,43 @@ def test_states_across_chunks_that_grow_or_fade_past_a_float(cuda_device, start,
     R.check(final, last, most_last, k, "final")
 
 
+@pytest.mark.parametrize("chunked", [False, True])
+def test_scan_without_a_skip_keeps_infinities(cuda_device, chunked):
+    """Without d, an infinite x gives what the states give, and an infinite gradient what they take: not 0 times infinity."""
+    inf = float("inf")
+    t, ch = (300, 3) if chunked else (40, 3)
+    x = torch.ones(t, ch, device="cuda")
+    dt, a = torch.ones(t, ch, device="cuda"), torch.full((ch, 8), -0.5, device="cuda")
+    b, c = torch.ones(t, 8, device="cuda"), torch.ones(t, 8, device="cuda")
+    x[t - 3, 1] = inf
+    y = torch.zeros_like(x)
+    room = _room(max(cuda_device.selective_scan_workspace(t, ch, 8), cuda_device.selective_scan_backward_workspace(t, ch, 8)))
+    marks = _room(cuda_device.selective_scan_checkpoints(t, ch, 8))
+    for ptr in (None, torch.tensor([0, t - 1], dtype=torch.int32).cuda()):  # whole batches, and an end inside one
+        cuda_device.selective_scan_device(x, dt, a, b, c, y, room, seq_ptr=ptr, checkpoints=marks, stream=_stream())
+        assert (y[t - 3:t - 1, 1] == inf).all() and torch.isfinite(y[:, [0, 2]]).all() and torch.isfinite(y[:t - 3]).all()
+    state = torch.zeros(1, ch, 8, device="cuda")
+    y1 = torch.zeros(1, ch, device="cuda")
+    cuda_device.selective_scan_step_device(x[t - 3:t - 2], dt[:1], a, b[:1], c[:1], y1, state, stream=_stream())
+    assert y1[0, 1] == inf
+    n = 2400
+    ym, xm = torch.zeros(n, 512, device="cuda"), torch.ones(n, 512, device="cuda")
+    xm[5, 7] = inf
+    am, one = torch.full((512, 8), -0.5, device="cuda"), torch.ones(n, 8, device="cuda")
+    cuda_device.selective_scan_step_device(xm, torch.ones_like(xm), am, one, one, ym, torch.zeros(n, 512, 8, device="cuda"),
+                                           stream=_stream())
+    assert ym[5, 7] == inf and torch.isfinite(ym).sum() == n * 512 - 1
+    x[t - 3, 1] = 1
+    dy = torch.ones_like(x)
+    dy[t - 3, 1] = inf
+    dx, ddt, da, db, dc = (torch.zeros_like(k) for k in (x, dt, a, b, c))
+    z = torch.ones_like(x)
+    cuda_device.selective_scan_device(x, dt, a, b, c, y, room, z=z, checkpoints=marks, stream=_stream())
+    dz = torch.zeros_like(x)
+    cuda_device.selective_scan_backward_device(dy, x, dt, a, b, c, marks, dx, ddt, da, db, dc, room, z=z, dz=dz, stream=_stream())
+    assert (dx[:t - 2, 1] == inf).all() and torch.isfinite(dx[t - 2:]).all() and torch.isfinite(dx[:, [0, 2]]).all()
+
+
 def test_scan_far_states(cuda_device):
     """A pool whose rows lie past 2^32 bytes and 2^31 values."""
     ch, ns, rows = 2048, 16, 70000
