@@ -531,6 +531,12 @@ uint64_t sparsl_selective_scan_checkpoints(uint64_t tokens, uint64_t channels, u
 int sparsl_dev_selective_scan_backward_device(sparsl_dev *dev, const sparsl_scan_args *args, void *stream);
 uint64_t sparsl_selective_scan_backward_workspace(uint64_t tokens, uint64_t channels, uint32_t states,
                                                   uint64_t n_seq, uint32_t groups);
+/* Test hook: how a pass over such tokens is laid out (ragged: with seq_ptr).
+ * out[5]: lanes a channel, chunks of the token axis, tokens of a chunk, whether
+ * states are handed on between chunks, and the lanes a channel of the pass that
+ * computes those (0: none). */
+int sparsl_selective_scan_test_layout(uint64_t tokens, uint64_t channels, uint32_t states, uint64_t n_seq,
+                                      uint32_t groups, int ragged, int backward, uint64_t *out);
 /* One token of each of n_seq sequences: the token arrays have n_seq rows;
  * final_state holds the states, updated in place. */
 int sparsl_dev_selective_scan_step_device(sparsl_dev *dev, const sparsl_scan_args *args, void *stream);

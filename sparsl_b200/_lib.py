@@ -176,6 +176,7 @@ SIGNATURES = {
     "sparsl_selective_scan_checkpoints": (u64, [u64, u64, u32]),
     "sparsl_dev_selective_scan_backward_device": (i32, [vp, vp, vp]),
     "sparsl_selective_scan_backward_workspace": (u64, [u64, u64, u32, u64, u32]),
+    "sparsl_selective_scan_test_layout": (i32, [u64, u64, u32, u64, u32, i32, i32, vp]),
     "sparsl_dev_selective_scan_step_device": (i32, [vp, vp, vp]),
     "sparsl_dev_layer_norm_device": (i32, [vp, vp, vp]),
     "sparsl_dev_layer_norm_backward_device": (i32, [vp, vp, vp]),

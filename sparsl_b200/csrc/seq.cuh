@@ -254,6 +254,14 @@ constexpr uint32_t kMaxStates = 64;
 size_t sscan_bytes(uint64_t tokens, uint64_t channels, uint32_t states, uint64_t n_seq, uint32_t groups);
 size_t sscan_backward_bytes(uint64_t tokens, uint64_t channels, uint32_t states, uint64_t n_seq, uint32_t groups);
 size_t sscan_mark_bytes(uint64_t tokens, uint64_t channels, uint32_t states);
+// How a pass is laid out, for tests: lanes a channel, chunks of the token axis and
+// their tokens, whether states are handed on between them, and the lanes a channel
+// of the pass in front that computes those (0: none).
+struct ScanLayout {
+  uint64_t lanes, chunks, len, carry, chunk_lanes;
+};
+ScanLayout sscan_layout(uint64_t tokens, uint32_t channels, uint32_t states, uint64_t n_seq, uint32_t groups, bool ragged);
+ScanLayout sscan_backward_layout(uint64_t tokens, uint32_t channels, uint32_t states, uint64_t n_seq, uint32_t groups, bool ragged);
 cudaError_t launch_sscan(const SscanArgs& a, cudaStream_t s);
 cudaError_t launch_sscan_backward(const SscanArgs& a, cudaStream_t s);
 cudaError_t launch_sscan_step(const SscanArgs& a, cudaStream_t s);

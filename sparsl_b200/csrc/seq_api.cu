@@ -535,6 +535,16 @@ uint64_t sparsl_selective_scan_backward_workspace(uint64_t tokens, uint64_t chan
   return sscan_backward_bytes(tokens, channels, states, n_seq, groups);
 }
 
+int sparsl_selective_scan_test_layout(uint64_t tokens, uint64_t channels, uint32_t states, uint64_t n_seq, uint32_t groups, int ragged,
+                                      int backward, uint64_t* out) {
+  if (!out || !channels || channels > (1u << 24) || !states || states > kMaxStates || !groups || channels % groups)
+    return SPARSL_ERR_INVALID;
+  const ScanLayout l = (backward ? sscan_backward_layout : sscan_layout)(tokens, (uint32_t)channels, states, n_seq, groups, ragged != 0);
+  const uint64_t v[5] = {l.lanes, l.chunks, l.len, l.carry, l.chunk_lanes};
+  for (int i = 0; i < 5; ++i) out[i] = v[i];
+  return SPARSL_OK;
+}
+
 int sparsl_dev_layer_norm_device(sparsl_dev* dev, const sparsl_norm_args* args, void* stream) {
   return norm(dev, args, stream, "layer_norm", FORWARD);
 }

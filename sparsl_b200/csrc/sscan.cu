@@ -19,6 +19,11 @@ size_t sscan_mark_bytes(uint64_t tokens, uint64_t channels, uint32_t states) {
   return (tokens + kMarkEvery - 1) / kMarkEvery * channels * states * 4;
 }
 
+ScanLayout sscan_layout(uint64_t tokens, uint32_t channels, uint32_t states, uint64_t n_seq, uint32_t groups, bool ragged) {
+  const ScanPlan p = scan_plan(tokens, channels, groups, n_seq, ragged, lanes_of(states));
+  return {p.lanes, p.chunks, p.len, p.carry, p.carry ? p.lanes : 0};
+}
+
 cudaError_t launch_sscan(const SscanArgs& a, cudaStream_t s) {
   switch (a.type) {
     case SEQ_F32: return launch_sscan_f32(a, s);

@@ -542,6 +542,22 @@ uint64_t back_work(const ScanPlan& p, uint64_t tokens, uint32_t channels, uint32
   return at + scan_round((uint64_t)p.per_group * tokens * groups * 2 * states * 4);
 }
 
+// The chunk pass keeps no history, so its lanes hold up to 16 states over the same
+// chunks; 4 where that leaves SMs with fewer than three blocks.
+constexpr uint32_t chunk_least(uint32_t padded) { return padded <= 16 ? 1 : padded / 16; }
+constexpr uint32_t chunk_most(uint32_t padded) { return padded <= 8 ? 2 : 4; }
+ScanPlan chunk_plan(ScanPlan p, uint32_t channels, uint32_t groups, uint32_t padded) {
+  const uint32_t cpg = channels / groups;
+  const auto lanes = [&](uint32_t k) {
+    p.lanes = k;
+    p.per_group = (cpg + kScanThreads / k - 1) / (kScanThreads / k);
+    p.ctiles = p.per_group * groups;
+  };
+  lanes(chunk_least(padded));
+  if (p.chunks * p.ctiles < 3 * kSms) lanes(chunk_most(padded));
+  return p;
+}
+
 template <class T, int NS, int LP, bool FULL, bool GATE>
 cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
   BackWork w{};
@@ -550,26 +566,15 @@ cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
   if (grid > 0x7fffffffull / 8 || cells / 256 >= 0x7fffffffull) return cudaErrorInvalidValue;
   cudaError_t e;
   if (p.carry) {
-    // The same chunks with up to 16 states a lane, as there is no history to keep;
-    // 4 where that leaves SMs with fewer than three blocks.
-    constexpr int NP = NS * LP, CL = NP <= 16 ? 1 : NP / 16, ML = NP <= 8 ? 2 : 4;
-    const uint32_t cpg = a.channels / a.groups;
-    ScanPlan q = p;
-    const auto lanes = [&](uint32_t k) {
-      q.lanes = k;
-      q.per_group = (cpg + kScanThreads / k - 1) / (kScanThreads / k);
-      q.ctiles = q.per_group * a.groups;
-      return p.chunks * q.ctiles;
-    };
-    uint64_t blocks = lanes(CL);
-    if (CL < ML && blocks < 3 * kSms) {
-      blocks = lanes(ML);
-      sscan_chunk_back_kernel<T, NP / ML, ML, FULL, GATE><<<(unsigned)blocks, kScanThreads, 0, s>>>(
+    constexpr int NP = NS * LP, CL = chunk_least(NP), ML = chunk_most(NP);
+    const ScanPlan q = chunk_plan(p, a.channels, a.groups, NP);
+    const unsigned blocks = (unsigned)(q.chunks * q.ctiles);
+    if (CL < ML && q.lanes == ML)
+      sscan_chunk_back_kernel<T, NP / ML, ML, FULL, GATE><<<blocks, kScanThreads, 0, s>>>(
           a, q, w.scan, rows_aligned<T, ML>(a, {{a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row}}));
-    } else {
-      sscan_chunk_back_kernel<T, NP / CL, CL, FULL, GATE><<<(unsigned)blocks, kScanThreads, 0, s>>>(
+    else
+      sscan_chunk_back_kernel<T, NP / CL, CL, FULL, GATE><<<blocks, kScanThreads, 0, s>>>(
           a, q, w.scan, rows_aligned<T, CL>(a, {{a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row}}));
-    }
     e = launch_sscan_fold_back(a.a, w.scan, p.chunks, a.channels, a.states, s);
     if (e != cudaSuccess) return e;
   }

@@ -290,6 +290,124 @@ def test_scan_many_sequences(cuda_device, shape):
         R.check(s.live(v) if name in ("dx", "ddt", "db", "dc", "dz") else v, *want[name], k, name)
 
 
+def _layout(tokens, ch, ns, n_seq, groups, ragged, backward):
+    """(lanes a channel, chunks, their tokens, states handed on, lanes of the pass that computes those)."""
+    import ctypes
+
+    from sparsl_b200 import _lib
+
+    out = (ctypes.c_uint64 * 5)()
+    assert _lib.load().sparsl_selective_scan_test_layout(tokens, ch, ns, n_seq, groups, ragged, backward, out) == 0
+    return list(out)
+
+
+def _part(s, seqs, groups):
+    """Some sequences and groups of a scan, as its oracle takes them: what they give does not depend on the others."""
+    import copy
+
+    per, at = s.ch // s.groups, R.lengths_to_ptr(s.lens)
+    rows = torch.cat([torch.arange(at[i], at[i + 1]) for i in seqs]).cuda()
+    cols = torch.cat([torch.arange(g * per, (g + 1) * per) for g in groups]).cuda()
+    p = copy.copy(s)
+    p.lens, p.ch, p.groups, p.lead = [s.lens[i] for i in seqs], len(cols), len(groups), 0
+    p.used = p.tokens = len(rows)
+    for k in ("x", "dt", "z", "dy"):
+        setattr(p, k, None if getattr(s, k) is None else s.live(getattr(s, k))[rows][:, cols])
+    p.b, p.c = (s.live(v)[rows][:, groups] for v in (s.b, s.c))
+    p.a, p.d, p.bias = (None if v is None else v[cols] for v in (s.a, s.d, s.bias))
+    p.state, p.dfinal = (None if v is None else v[list(seqs)][:, cols] for v in (s.state, s.dfinal))
+    return p, rows, cols
+
+
+# Sizes at which a scan takes the layouts that large inputs take: one of few lanes a channel with states handed on, and whole
+# sequences with two lanes.  `ahead` is the layout of the prompt, `back` of the gradients: lanes, handed on, the chunk pass's lanes.
+MANY = [70, 1300, 0, 1, 64, 129, 3]
+LARGE = [
+    dict(lens=MANY, ns=16, dtype=torch.bfloat16, ahead=(1, 1, 1), back=(2, 1, 4)),
+    dict(lens=MANY, ns=16, dtype=torch.float16, ahead=(1, 1, 1), back=(2, 1, 4)),
+    dict(lens=MANY, ns=11, dtype=torch.float32, ahead=(1, 1, 1), back=(2, 1, 4)),
+    dict(lens=MANY, ns=8, dtype=torch.bfloat16, ahead=(1, 1, 1), back=(1, 1, 1)),
+    dict(lens=MANY, ns=5, dtype=torch.float32, ahead=(1, 1, 1), back=(1, 1, 1), gate=False),
+    dict(lens=MANY, ns=32, dtype=torch.bfloat16, ahead=(2, 1, 2), back=(4, 1, 4)),
+    dict(lens=MANY, ns=23, dtype=torch.float16, ahead=(2, 1, 2), back=(4, 1, 4), gate=False),
+    dict(lens=MANY, ns=64, dtype=torch.bfloat16, ahead=(4, 1, 4), back=(8, 1, 4)),
+    dict(lens=[96] * 8, ns=16, dtype=torch.bfloat16, ahead=(2, 0, 0), back=(2, 0, 0), ragged=False, ch=2048, groups=16),
+    dict(lens=[96] * 8, ns=13, dtype=torch.float32, ahead=(2, 0, 0), back=(2, 0, 0), ragged=False, ch=2048, groups=16),
+]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: f"{c['ns']}-{str(c['dtype'])[6:]}-{'-'.join(map(str, c['ahead'] + c['back']))}")
+def test_scan_layouts_of_large_inputs(cuda_device, case):
+    case = dict(case)
+    ahead, back = case.pop("ahead"), case.pop("back")
+    ragged = case.get("ragged", True)
+    case = {"ch": 4096, "groups": 32, "lead": 2 * ragged, "tail": 5 * ragged, **case}
+    s = Scan(state=True, **case)
+    n = len(s.lens)
+    for want, b in ((ahead, False), (back, True)):
+        lanes, chunks, _, carry, first = _layout(s.tokens, s.ch, s.ns, n, s.groups, ragged, b)
+        assert (lanes, carry, first) == want and (chunks > 1 or not carry)
+    marks = s.marks(cuda_device)
+    final = torch.full_like(s.state, NAN)
+    y = s.forward(cuda_device, marks=marks, state=s.state, final=final)
+    got = s.backward(cuda_device, marks)
+    # In place, in a pool by slot; one sequence begins anew, one keeps no state.
+    slots = torch.randperm(n + 3, generator=_gen(4))[:n].to(torch.int32)
+    slots[0] = -1
+    resume = torch.ones(n, dtype=torch.uint8)
+    resume[1] = 0
+    pool = torch.full((n + 3, s.ch, s.ns), 3.0, device="cuda")
+    pool[slots[1:].long().cuda()] = s.state[1:]
+    y2 = s.forward(cuda_device, state=pool, final=pool, slots=slots.cuda(), resume=resume.cuda())
+    s.untouched(y)
+    s.untouched(y2)
+    groups = [0, s.groups // 2, s.groups - 1]
+    p, rows, cols = _part(s, range(n), groups)
+    want, k = p.oracle(p.state, backward=True)
+    pick = lambda v: s.live(v)[:, cols]  # noqa: E731
+    R.check(pick(y), *want["y"], k, "y")
+    R.check(final[:, cols], *want["final"], k, "final")
+    for name, v in got.items():
+        if name in ("db", "dc"):
+            v = s.live(v)[:, groups]
+        elif name in ("dx", "ddt", "dz"):
+            s.untouched(v)
+            v = pick(v)
+        else:
+            v = v[:, cols] if name == "dstate" else v[cols]
+        R.check(v, *want[name], k, name)
+    start = p.state.clone()
+    start[:2] = 0
+    want, k = p.oracle(start)
+    R.check(pick(y2), *want["y"], k, "y, in place")
+    kept = slots[1:].long()
+    R.check(pool[kept.cuda()][:, cols], *(v[1:] for v in want["final"]), k, "pool")
+    rest = [r for r in range(n + 3) if r not in slots.tolist()]
+    assert (pool[rest] == 3).all()
+
+
+def test_scan_of_very_many_chunks(cuda_device):
+    """One tile of channels over hundreds of chunks, where the gradients' chunk pass takes one lane a channel; the first, the
+    last and a long sequence against the formulas."""
+    lens = [900, 3, 1, 40] + [1300] * 21 + [300, 64]
+    s = Scan(lens, 64, 16, dtype=torch.bfloat16, state=True)
+    assert _layout(s.tokens, 64, 16, len(lens), 1, True, False)[3:] == [1, 1]
+    lanes, chunks, _, carry, first = _layout(s.tokens, 64, 16, len(lens), 1, True, True)
+    assert (lanes, carry, first) == (2, 1, 1) and chunks >= 444
+    marks = s.marks(cuda_device)
+    final = torch.full_like(s.state, NAN)
+    y = s.forward(cuda_device, marks=marks, state=s.state, final=final)
+    got = s.backward(cuda_device, marks)
+    seqs = [0, 3, 14, len(lens) - 1]
+    p, rows, _ = _part(s, seqs, [0])
+    want, k = p.oracle(p.state, backward=True)
+    R.check(y[rows], *want["y"], k, "y")
+    R.check(final[seqs], *want["final"], k, "final")
+    for name in ("dx", "ddt", "db", "dc", "dz"):
+        R.check(got[name][rows], *want[name], k, name)
+    R.check(got["dstate"][seqs], *want["dstate"], k, "dstate")
+
+
 def test_scan_infinite_and_nan_stay_in_their_sequence(cuda_device):
     s = Scan([50, 40, 60], 20, 11)
     clean = s.forward(cuda_device)
@@ -361,6 +479,40 @@ def test_scan_without_a_skip_keeps_infinities(cuda_device, chunked):
     dz = torch.zeros_like(x)
     cuda_device.selective_scan_backward_device(dy, x, dt, a, b, c, marks, dx, ddt, da, db, dc, room, z=z, dz=dz, stream=_stream())
     assert (dx[:t - 2, 1] == inf).all() and torch.isfinite(dx[t - 2:]).all() and torch.isfinite(dx[:, [0, 2]]).all()
+
+
+@pytest.mark.parametrize("ns,ragged", [(16, True), (16, False), (5, False)])
+def test_scan_long_memory_is_not_biased(cuda_device, ns, ragged):
+    """States that only fade, over 1024 tokens: their mean relative error stays below 1e-8 a token, half of what the special
+    function unit's powers of two alone are low by, and 1e-6 for the mean of the roundings; with a step of zero the bits stay."""
+    t, ch = 1024, 64
+    g = _gen(3)
+    # s a in (-0.06, 0), so that the states end above exp(-62) of their start.
+    dt, a = torch.rand(t, ch, generator=g) * 0.06, -torch.rand(ch, ns, generator=g)
+    state = 1 + torch.rand(1, ch, ns, generator=g)
+    final = torch.zeros(1, ch, ns, device="cuda")
+    zero = torch.zeros(t, ch, device="cuda")
+    room = _room(cuda_device.selective_scan_workspace(t, ch, ns))
+    ptr = torch.tensor([0, t], dtype=torch.int32).cuda() if ragged else None
+
+    def run(dt):
+        cuda_device.selective_scan_device(zero, dt, a.cuda(), torch.zeros(t, ns, device="cuda"), torch.zeros(t, ns, device="cuda"),
+                                          torch.zeros_like(zero), room, seq_ptr=ptr, state=state.cuda(), final_state=final,
+                                          stream=_stream())
+        return _up(final[0])
+
+    want = _up(state[0]) * torch.exp(_up(dt).sum(0)[:, None] * _up(a))
+    off = run(dt.cuda()) / want - 1
+    assert abs(float(off.mean())) < t * 1e-8 + 1e-6, float(off.mean())
+    assert torch.equal(run(zero), _up(state[0]))
+    pool = state.cuda()  # token by token
+    row = torch.zeros(1, ns, device="cuda")
+    steps = dt.cuda()
+    for k in range(t):
+        cuda_device.selective_scan_step_device(zero[:1], steps[k:k + 1], a.cuda(), row, row, torch.zeros(1, ch, device="cuda"), pool,
+                                               stream=_stream())
+    off = _up(pool[0]) / want - 1
+    assert abs(float(off.mean())) < t * 1e-8 + 1e-6, float(off.mean())
 
 
 def test_scan_far_states(cuda_device):

@@ -159,3 +159,23 @@ def test_a_handle_is_the_stream_it_comes_from():
     from sparsl_b200.sequence import _stream
 
     assert _stream(0) == 1 == _stream(types.SimpleNamespace(cuda_stream=0)) and _stream(1) == 1 and _stream(None) is None
+
+
+def test_layouts_of_the_scan():
+    """Large prompts take one lane a channel and hand states on; whole sequences that fill two fifths of a wave of blocks do not."""
+    import ctypes
+
+    def layout(*args):
+        out = (ctypes.c_uint64 * 5)()
+        assert _lib.load().sparsl_selective_scan_test_layout(*args, out) == 0
+        return list(out)
+
+    lanes, chunks, length, carry, first = layout(32768, 2048, 16, 1, 1, 0, 0)
+    assert (lanes, carry, first) == (1, 1, 1) and (chunks - 1) * length < 32768 <= chunks * length and length % 32 == 0
+    assert layout(16384, 2048, 16, 8, 1, 0, 0) == [2, 8, 2048, 0, 0]
+    assert layout(16384, 2048, 16, 8, 1, 0, 1) == [2, 8, 2048, 0, 0]
+    assert layout(16384, 2048, 16, 8, 1, 1, 1)[3] == 1  # unequal ones are cut
+    assert layout(0, 8, 4, 1, 1, 0, 0)[1:2] == [1]
+    bad = (ctypes.c_uint64 * 5)()
+    for args in ((8, 0, 4, 1, 1, 0, 0), (8, 9, 4, 1, 2, 0, 0), (8, 8, 65, 1, 1, 0, 0), (8, 8, 0, 1, 1, 0, 1)):
+        assert _lib.load().sparsl_selective_scan_test_layout(*args, bad) != 0
