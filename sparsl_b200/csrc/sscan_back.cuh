@@ -542,19 +542,15 @@ uint64_t back_work(const ScanPlan& p, uint64_t tokens, uint32_t channels, uint32
   return at + scan_round((uint64_t)p.per_group * tokens * groups * 2 * states * 4);
 }
 
-// The chunk pass keeps no history, so its lanes hold up to 16 states over the same
-// chunks; 4 where that leaves SMs with fewer than three blocks.
-constexpr uint32_t chunk_least(uint32_t padded) { return padded <= 16 ? 1 : padded / 16; }
-constexpr uint32_t chunk_most(uint32_t padded) { return padded <= 8 ? 2 : 4; }
+// The chunk pass takes the same chunks with 4 states a lane, of 64 with 16: its
+// blocks are few.  With 16 states a lane wherever that leaves three blocks an SM
+// the gradients' calls took 187 us against 175 (28,600 unequal tokens x 64 channels
+// x 16 states), 886 against 877 (10,400 x 4096 x 8), 74 against 71 (700 x 2048 x 8).
+constexpr uint32_t chunk_lanes(uint32_t padded) { return padded <= 8 ? 2 : 4; }
 ScanPlan chunk_plan(ScanPlan p, uint32_t channels, uint32_t groups, uint32_t padded) {
-  const uint32_t cpg = channels / groups;
-  const auto lanes = [&](uint32_t k) {
-    p.lanes = k;
-    p.per_group = (cpg + kScanThreads / k - 1) / (kScanThreads / k);
-    p.ctiles = p.per_group * groups;
-  };
-  lanes(chunk_least(padded));
-  if (p.chunks * p.ctiles < 3 * kSms) lanes(chunk_most(padded));
+  p.lanes = chunk_lanes(padded);
+  p.per_group = (channels / groups + kScanThreads / p.lanes - 1) / (kScanThreads / p.lanes);
+  p.ctiles = p.per_group * groups;
   return p;
 }
 
@@ -566,15 +562,10 @@ cudaError_t go(const SscanArgs& a, const ScanPlan& p, cudaStream_t s) {
   if (grid > 0x7fffffffull / 8 || cells / 256 >= 0x7fffffffull) return cudaErrorInvalidValue;
   cudaError_t e;
   if (p.carry) {
-    constexpr int NP = NS * LP, CL = chunk_least(NP), ML = chunk_most(NP);
+    constexpr int NP = NS * LP, CL = chunk_lanes(NP);
     const ScanPlan q = chunk_plan(p, a.channels, a.groups, NP);
-    const unsigned blocks = (unsigned)(q.chunks * q.ctiles);
-    if (CL < ML && q.lanes == ML)
-      sscan_chunk_back_kernel<T, NP / ML, ML, FULL, GATE><<<blocks, kScanThreads, 0, s>>>(
-          a, q, w.scan, rows_aligned<T, ML>(a, {{a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row}}));
-    else
-      sscan_chunk_back_kernel<T, NP / CL, CL, FULL, GATE><<<blocks, kScanThreads, 0, s>>>(
-          a, q, w.scan, rows_aligned<T, CL>(a, {{a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row}}));
+    sscan_chunk_back_kernel<T, NP / CL, CL, FULL, GATE><<<(unsigned)(q.chunks * q.ctiles), kScanThreads, 0, s>>>(
+        a, q, w.scan, rows_aligned<T, CL>(a, {{a.dt, a.dt_row}, {a.dy, a.dy_row}, {a.z, a.z_row}}));
     e = launch_sscan_fold_back(a.a, w.scan, p.chunks, a.channels, a.states, s);
     if (e != cudaSuccess) return e;
   }
