@@ -26,10 +26,11 @@ struct ScanPlan {
 };
 
 // How many lanes share a channel's states: `least` is what the registers
-// demand, up to `most`; the blocks that an SM holds; and how full, in
-// twentieths, whole sequences have to make their waves of blocks.
+// demand, up to `most`; the blocks that an SM holds; the states, with those that
+// pad them; and how full, in twentieths, whole sequences have to make their waves of
+// blocks (`thin`: with lanes of 4 states; above 20: never).
 struct ScanLanes {
-  uint32_t least, most, resident, fill;
+  uint32_t least, most, resident, states, fill, thin;
 };
 
 inline ScanPlan scan_plan(uint64_t tokens, uint32_t channels, uint32_t groups, uint64_t n_seq, bool ragged, ScanLanes l) {
@@ -42,7 +43,7 @@ inline ScanPlan scan_plan(uint64_t tokens, uint32_t channels, uint32_t groups, u
   // the first pass, and leave their SMs to others); more lanes a channel where
   // that leaves SMs with fewer than three quarters of their blocks.
   for (uint32_t k = l.least; k <= l.most; k *= 2) {
-        const uint64_t ct = (uint64_t)groups * tiles(k), some = ragged ? 2 * slots : slots, want = ct >= some ? 1 : some / ct;
+    const uint64_t ct = (uint64_t)groups * tiles(k), some = ragged ? 2 * slots : slots, want = ct >= some ? 1 : some / ct;
     p.lanes = k;
     p.len = (tokens + want - 1) / want;
     p.len = p.len < 64 ? 64 : (p.len + 31) / 32 * 32;
@@ -51,14 +52,21 @@ inline ScanPlan scan_plan(uint64_t tokens, uint32_t channels, uint32_t groups, u
   }
   p.carry = p.chunks > 1;
   // Whole sequences instead, in one pass without the states at the chunks'
-  // starts, where they fill enough of their waves of blocks: two fifths in the
-  // forward pass, whose chunks take nearly twice the time (1.34 ms a training step
-  // against 1.37 at 8 sequences x 2048 channels, 256 blocks), three quarters in
-  // the backward pass, whose first pass over the chunks is a fifth of it.
+  // starts, where they fill enough of their waves of blocks.  Measured in us, whole
+  // sequences against chunks, bf16 tokens x 2048 channels (share of the waves):
+  // Prompts, whose chunks take nearly twice the work, from two fifths on: 16 states,
+  // 7 x 2048 tokens (0.38) 357 : 356, 8 x 2048 (0.43) 356 : 381, 8 x 512 96 : 124; 8
+  // states, 12 x 1024 (0.32) 200 : 200; 32 states, 6 x 1024 (0.32) 286 : 295; 64 states,
+  // 1024 channels, 7 x 1024 (0.38) 486 : 452, 8 x 1024 (0.43) 486 : 513.  With 4 states
+  // a lane from three fifths on: 4 x 2048 (0.43) 292 : 205, 6 x 2048 (0.65) 327 : 304,
+  // 6 x 512 88 : 100, f32 6 x 1024 162 : 180.
+  // Gradients, whose first pass over the chunks is a fifth of it, from four fifths
+  // on: 7 x 2048 (0.76) 977 : 948, 8 x 2048 (0.86) 979 : 1070, 12 x 2048 (0.65 of two
+  // waves) 1702 : 1513; never with 4 states a lane: 4 x 2048 (0.86) 774 : 582.
   if (!ragged && run && run % 32 == 0)
     for (uint32_t k = l.least; k <= l.most; k *= 2) {
       const uint64_t blocks = n_seq * groups * tiles(k), waves = (blocks + slots - 1) / slots;
-      if (20 * blocks < l.fill * waves * slots && run > 64) continue;
+      if (20 * blocks < (l.states / k == 4 ? l.thin : l.fill) * waves * slots && run > 64) continue;
       p.lanes = k;
       p.len = run;
       p.chunks = n_seq;

@@ -523,7 +523,7 @@ bool aligned16(const void* p) { return reinterpret_cast<uint64_t>(p) % 16 == 0; 
 // x 2048 channels x 16 states, but this kernel 41 us against 65 at 1531 x 402 x 11.
 ScanLanes lanes_of(uint32_t states) {
   const uint32_t least = states <= 8 ? 1 : states <= 16 ? 2 : states <= 32 ? 4 : 8;
-  return {least, least == 8 ? 8 : 2 * least, (uint32_t)resident(8), 15u};
+  return {least, least == 8 ? 8 : 2 * least, (uint32_t)resident(8), 8 * least, 16u, 21u};
 }
 
 ScanPlan plan_of(uint64_t tokens, uint32_t channels, uint32_t states, uint64_t n_seq, uint32_t groups, bool ragged) {
@@ -542,8 +542,8 @@ uint64_t back_work(const ScanPlan& p, uint64_t tokens, uint32_t channels, uint32
   return at + scan_round((uint64_t)p.per_group * tokens * groups * 2 * states * 4);
 }
 
-// The chunk pass takes the same chunks with 4 states a lane, of 64 with 16: its
-// blocks are few.  With 16 states a lane wherever that leaves three blocks an SM
+// The chunk pass takes the same chunks with 4 states a lane (8 of 32, 16 of 64):
+// its blocks are few.  With 16 states a lane wherever that leaves three blocks an SM
 // the gradients' calls took 187 us against 175 (28,600 unequal tokens x 64 channels
 // x 16 states), 886 against 877 (10,400 x 4096 x 8), 74 against 71 (700 x 2048 x 8).
 constexpr uint32_t chunk_lanes(uint32_t padded) { return padded <= 8 ? 2 : 4; }

@@ -438,7 +438,7 @@ bool aligned16(const void* p) { return reinterpret_cast<uint64_t>(p) % 16 == 0; 
 constexpr uint32_t padded(uint32_t states) { return states <= 8 ? 8 : states <= 16 ? 16 : states <= 32 ? 32 : 64; }
 ScanLanes lanes_of(uint32_t states) {
   const uint32_t np = padded(states);
-  return {np <= 16 ? 1u : np / 16, np <= 8 ? 2u : 4u, kResident, 8u};
+  return {np <= 16 ? 1u : np / 16, np <= 8 ? 2u : 4u, kResident, np, 8u, 12u};
 }
 
 ScanPlan plan_of(const SscanArgs& a) {

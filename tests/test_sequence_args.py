@@ -175,6 +175,9 @@ def test_layouts_of_the_scan():
     assert layout(16384, 2048, 16, 8, 1, 0, 0) == [2, 8, 2048, 0, 0]
     assert layout(16384, 2048, 16, 8, 1, 0, 1) == [2, 8, 2048, 0, 0]
     assert layout(16384, 2048, 16, 8, 1, 1, 1)[3] == 1  # unequal ones are cut
+    for n, back in ((4, 0), (5, 0), (4, 1), (7, 1), (12, 1)):  # whole ones with 4 states a lane, or in waves that stay empty, are slower
+        assert layout(n * 2048, 2048, 16, n, 1, 0, back)[3] == 1
+    assert layout(7 * 1024, 1024, 64, 7, 1, 0, 0)[3] == 1 and layout(8 * 1024, 1024, 64, 8, 1, 0, 0)[3] == 0
     assert layout(0, 8, 4, 1, 1, 0, 0)[1:2] == [1]
     bad = (ctypes.c_uint64 * 5)()
     for args in ((8, 0, 4, 1, 1, 0, 0), (8, 9, 4, 1, 2, 0, 0), (8, 8, 65, 1, 1, 0, 0), (8, 8, 0, 1, 1, 0, 1)):
