@@ -2,8 +2,9 @@
 convolution, the selective state space scan and layer norm (``sparsl_dev_*_device``
 in include/sparsl_cuda.h, which states their formulas).
 
-Arrays are device arrays of the device's GPU: torch tensors, or objects with
-``data_ptr()``, ``shape``, ``stride()`` and ``dtype``.  Token arrays are
+Arrays are device arrays of the device's GPU: torch tensors, or objects with a
+tensor's ``data_ptr()``, ``shape`` (a tuple), ``stride()``, ``dtype``,
+``is_contiguous()``, ``numel()`` and ``element_size()``.  Token arrays are
 [tokens, channels] with the channels next to each other; rows may be strided, so
 column ranges of a wider array serve as they are.  Every call only enqueues its
 work: on ``stream`` (a cudaStream_t, 0 the legacy default stream, or a torch

@@ -936,6 +936,84 @@ def test_other_streams(cuda_device):
     assert torch.equal(y1, y2) and torch.equal(y1, y3)
 
 
+def test_far_token_rows(cuda_device):
+    """Convolution and scan, forward and gradients, over column ranges of arrays whose rows pass 2^32 bytes and 2^31 values
+    give the bits that they give over contiguous rows."""
+    dev, st = cuda_device, _stream()
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("the rows do not fit this GPU")
+    t, ch, ns, dtype = 36000, 32, 8, torch.bfloat16
+    g = _gen(6)
+    lens = [9000, 1, 26900]  # 99 rows of no sequence
+    ptr = torch.tensor(R.lengths_to_ptr(lens), dtype=torch.int32).cuda()
+    wide = torch.zeros(t, 65536, dtype=dtype, device="cuda")
+    far = [wide[:, 800 * 64 + k * 64:][:, :ch] for k in range(10)]  # x, dt, z, dy, y, dx, ddt, dz, v, dv
+    near = [torch.zeros(t, ch, dtype=dtype, device="cuda") for _ in far]
+    for k in range(4):
+        near[k].copy_(torch.randn(t, ch, generator=g))
+        far[k].copy_(near[k])
+    b, c = torch.randn(t, ns, generator=g).to(dtype).cuda(), torch.randn(t, ns, generator=g).to(dtype).cuda()
+    a, w = -torch.rand(ch, ns, generator=g).cuda() - 0.5, torch.randn(ch, 4, generator=g).cuda()
+    marks = _room(dev.selective_scan_checkpoints(t, ch, ns))
+    room = _room(max(dev.selective_scan_workspace(t, ch, ns, 3), dev.selective_scan_backward_workspace(t, ch, ns, 3),
+                     dev.causal_conv_backward_workspace(t, ch, 4)))
+
+    def run(x, dt, z, dy, y, dx, ddt, dz, v, dv):
+        da, db, dc, dw = torch.empty_like(a), torch.zeros_like(b), torch.zeros_like(c), torch.empty_like(w)
+        dev.causal_conv_device(x, w, v, silu=True, seq_ptr=ptr, stream=st)
+        dev.selective_scan_device(v, dt, a, b, c, y, room, z=z, softplus=True, seq_ptr=ptr, checkpoints=marks, stream=st)
+        dev.selective_scan_backward_device(dy, v, dt, a, b, c, marks, dv, ddt, da, db, dc, room, z=z, dz=dz, softplus=True,
+                                           seq_ptr=ptr, stream=st)
+        dev.causal_conv_backward_device(dv, x, w, dx, dw, room, silu=True, seq_ptr=ptr, stream=st)
+        return da, db, dc, dw
+
+    first, second = run(*near), run(*far)
+    for p, q in zip((*near, *first), (*far, *second)):
+        assert torch.equal(p, q) and torch.isfinite(p).all()
+    assert far[4][30000:35000].abs().max() > 0 and (far[4][sum(lens):] == 0).all()
+    del wide, far, p, q
+    torch.cuda.empty_cache()
+
+
+def test_replayed_with_other_sequences(cuda_device):
+    """A captured prompt reads seq_ptr, slots and resume when it runs: replayed with others it gives what a call with them gives."""
+    dev = cuda_device
+    s, v = Scan([90, 0, 130, 40, 60], 72, 16, dtype=torch.bfloat16), Conv([90, 0, 130, 40, 60], 72, 4, torch.bfloat16)
+    slots, resume = torch.tensor([3, 0, 5, 1, 6], dtype=torch.int32).cuda(), torch.tensor([1, 0, 1, 0, 1], dtype=torch.uint8).cuda()
+    pool, cpool = torch.randn(8, 72, 16, device="cuda"), torch.randn(8, 3, 72, device="cuda").to(torch.bfloat16)
+    keep = pool.clone(), cpool.clone()
+    y, u = torch.zeros_like(s.x), torch.zeros_like(s.x)
+    room = _room(dev.selective_scan_workspace(s.tokens, 72, 16, 5, 1))
+
+    def run():
+        st = torch.cuda.current_stream()
+        dev.causal_conv_device(v.x, v.w, u, bias=v.bias, seq_ptr=s.ptr, state=cpool, final_state=cpool, slots=slots, resume=resume,
+                               stream=st)
+        dev.selective_scan_device(u, s.dt, s.a, s.b, s.c, y, room, d=s.d, z=s.z, dt_bias=s.bias, softplus=True, seq_ptr=s.ptr,
+                                  state=pool, final_state=pool, slots=slots, resume=resume, stream=st)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for starts, rows, begin in (([0, 90, 90, 220, 260, 320], [3, 0, 5, 1, 6], [1, 0, 1, 0, 1]),
+                                ([2, 3, 200, 200, 201, 310], [0, -1, 7, 2, 4], [0, 1, 1, 1, 0]),
+                                ([0, 0, 0, 320, 320, 320], [1, 2, 3, 4, 5], [1, 1, 1, 1, 1])):
+        s.ptr.copy_(torch.tensor(starts))
+        slots.copy_(torch.tensor(rows))
+        resume.copy_(torch.tensor(begin))
+        got = []
+        for go in (graph.replay, run):
+            pool.copy_(keep[0])
+            cpool.copy_(keep[1])
+            y.fill_(7)
+            u.fill_(7)
+            go()
+            torch.cuda.synchronize()
+            got.append([t.clone() for t in (y, u, pool, cpool)])
+        assert all(torch.equal(p, q) for p, q in zip(*got))
+        assert (got[0][0][:starts[0]] == 7).all() and (got[0][0][starts[-1]:] == 7).all()
+
+
 def test_the_default_streams_handle_is_that_stream(cuda_device):
     """A call on the handle of torch's default stream, 0, follows the work that makes its inputs there."""
     x, y = torch.zeros(4096, 4096, device="cuda"), torch.zeros(4096, 4096, device="cuda")
