@@ -7,7 +7,9 @@
 // first token, or zeros.  All of it is bound by HBM: x read and y written once.
 // Measured at 16384 packed tokens x 4096 channels, width 4 with the sigmoid, bf16:
 // 55 us, 4.9 TB/s; the two special functions a value alone take 30 us of the 42
-// that HBM does.
+// that HBM does.  The gradients of the same size take 418 us in bf16, 315 in f16 and
+// 224 in f32, whose bytes take 62 and 125: at 177, 158 and 114 registers a thread an SM
+// holds two, three and four blocks, and the times go with that.
 #include "seq.cuh"
 
 namespace sparsl {

@@ -5,14 +5,16 @@
 //   dw  = sum over rows of dy hat,   dbias = sum over rows of dy
 //
 // Bound by HBM: forward x read and y written once, backward x and dy read and
-// dx written once.  A group of threads keeps a row in registers (32 values a
+// dx written once.  A group of threads keeps a row in registers (64 values a
 // thread at most), so the variance is the mean of squared deviations, not a
 // difference of sums; longer rows are read again for each of the steps.  In
 // the backward pass a block walks many rows, its threads keeping the sums of dw
 // and dbias for their own channels in registers, and the blocks' partial rows
 // are added in a fixed order.  Measured at 16384 x 2048 bf16: forward 36 us (3.7
 // TB/s), backward 48 us (4.2 TB/s) and 8 us for the partial rows; at 4099 x 5003
-// f32, rows that no 16-byte access fits, 45 and 62 us (3.6 and 3.9 TB/s).
+// f32, rows that no 16-byte access fits, 45 and 62 us (3.6 and 3.9 TB/s).  The
+// gradients of rows over 8192 values read x and dy twice in one kernel and once in
+// another, value by value: 479 us at 8192 x 12288 bf16, whose bytes take 94.
 #include "seq.cuh"
 
 namespace sparsl {

@@ -195,8 +195,7 @@ __device__ __forceinline__ float dot(const float* c, const f32x2 (&h)[NS / 2]) {
 // The main pass over one chunk, in batches of eight tokens.  A batch inside one
 // sequence takes the straight path; one in which a sequence begins or ends
 // elsewhere than at its edges goes token by token.  128 registers a thread, 16
-// warps an SM: 20 or 24 warps with fewer rows in flight were slower (813 and 842
-// us against 776 for the whole scan, in an earlier form).
+// warps an SM: a lane holds its states, their exponents and two tokens' decays.
 template <class T, int NS, int LP, bool FULL, bool GATE>
 __global__ void __launch_bounds__(kScanThreads, kResident) sscan_kernel(SscanArgs a, ScanPlan p, ScanWork w, int aligned) {
   constexpr int NP = NS * LP, K = kBatch, kOwn = K / LP, A = GATE ? 3 : 2;
