@@ -142,7 +142,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // 2^v and 1/v by the special function unit (relative error below 2^-22 and
 // 2^-23): the sums they enter are rounded at 2^-24 a step, and the outputs
-// they reach at most at that of f32.
+// they reach at most at that of f32.  Results below 2^-126 are zero: a state that
+// one token takes that far down is gone.
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
